@@ -383,6 +383,51 @@ typedef struct snr_adam_pack_item {
 int snr_adam_pack_multi(const snr_adam_pack_item* items, int n_items, float lr, float beta1, float beta2, float eps, int step,
                         float grad_scale, const snr_step_state* state, snr_stream_t stream);
 
+/* Adam on a list of tensors in ONE launch (48 tensors a launch): the update of snr_adam_step, bit for bit, on ranges that do not
+ * touch each other — what of a network is no hidden matrix (input layer, heads, biases) when snr_muon_step_multi takes the rest.
+ * state NULL: rate `lr` and bias corrections from `step` (1-based); else both are read from the device-side snr_step_state.
+ * Items with n == 0 are skipped. */
+typedef struct snr_adam_item {
+  float* params;
+  const float* grads;
+  float* exp_avg;
+  float* exp_avg_sq;
+  int64_t n;
+} snr_adam_item;
+int snr_adam_step_multi(const snr_adam_item* items, int n_items, float lr, float beta1, float beta2, float eps, int step,
+                        float grad_scale, const snr_step_state* state, snr_stream_t stream);
+
+/* ---- orthogonalised updates (Newton-Schulz products), for the hidden matrices of a network ----
+ * out = X_steps with X_0 = x / max(|x|_F, eps), A = X X^T, X <- a X + (b A + c A A) X, for every matrix of a stack [batch, rows,
+ * cols] of fp32 / fp16 / bf16 whose columns are contiguous (row and matrix strides in elements).  `out` may be x itself.
+ * precision: SNR_ORTH_FP32 carries every product at fp32's accuracy, SNR_ORTH_FP16 multiplies fp16 roundings (2^-11) with fp32
+ * sums (where the shorter side is above 64: below, both are the same); X itself has 22 bits in either.  a, b, c must keep singular values from [0, 1] below 8 over `steps`, and |b l + c l^2|
+ * below 64 on the way (SNR_ERR_UNSUPPORTED otherwise).  A matrix that is all zero gives zeros; one with a NaN or an infinity
+ * gives NaN throughout.  Results do not depend on the stack around a matrix and repeat bit for bit. */
+enum { SNR_F32 = 0, SNR_F16 = 1, SNR_BF16 = 2 };
+enum { SNR_ORTH_FP16 = 0, SNR_ORTH_FP32 = 1 };
+int64_t snr_orthogonalise_ws_bytes(int64_t batch, int64_t rows, int64_t cols, int precision);
+int snr_orthogonalise(const void* x, int dtype, int64_t batch, int64_t rows, int64_t cols, int64_t x_batch_stride,
+                      int64_t x_row_stride, void* out, int64_t out_batch_stride, int64_t out_row_stride, int steps, float a, float b,
+                      float c, float eps, int precision, void* ws, snr_stream_t stream);
+
+/* The optimizer step around it, for a list of stacks (contiguous fp32 [batch, rows, cols]):
+ *   momentum <- mu momentum + grad_scale g;   u = grad_scale g + mu momentum (nesterov) or momentum;
+ *   params <- params (1 - lr weight_decay) - lr q orthogonalise(u)
+ * q = 1, sqrt(max(1, rows / cols)) or 0.2 sqrt(max(rows, cols)) (SNR_MUON_NONE / _SPECTRAL / _RMS).  params and momentum of the
+ * items must not overlap.  state: as above (only the rate is read). */
+enum { SNR_MUON_NONE = 0, SNR_MUON_SPECTRAL = 1, SNR_MUON_RMS = 2 };
+typedef struct snr_muon_item {
+  float* params;
+  const float* grads;
+  float* momentum;
+  int64_t batch, rows, cols;
+} snr_muon_item;
+int64_t snr_muon_ws_bytes(const snr_muon_item* items, int n_items, int precision);
+int snr_muon_step_multi(const snr_muon_item* items, int n_items, float lr, float momentum, int nesterov, float weight_decay,
+                        int scale_mode, int steps, float a, float b, float c, float eps, float grad_scale, int precision,
+                        const snr_step_state* state, void* ws, snr_stream_t stream);
+
 /* ---- diagnostics: per-kernel HIP-event timing (used by bench.py for the roofline line) ----
  * When enabled, every kernel launch of this library is bracketed by hipEvents on its stream;
  * snr_prof_read() waits for them, returns total elapsed ms and launch count per kernel id

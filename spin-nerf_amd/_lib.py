@@ -75,6 +75,18 @@ class AdamPackItem(_c.Structure):   # snr_adam_pack_item
     _fields_ = [("cfg", _CFG), ("params", _p), ("grads", _p), ("exp_avg", _p), ("exp_avg_sq", _p), ("packed", _p)]
 
 
+class AdamItem(_c.Structure):       # snr_adam_item
+    _fields_ = [("params", _p), ("grads", _p), ("exp_avg", _p), ("exp_avg_sq", _p), ("n", _l)]
+
+
+class MuonItem(_c.Structure):       # snr_muon_item
+    _fields_ = [("params", _p), ("grads", _p), ("momentum", _p), ("batch", _l), ("rows", _l), ("cols", _l)]
+
+
+F32, F16, BF16 = 0, 1, 2                              # SNR_F32 ...
+ORTH_FP16, ORTH_FP32 = 0, 1                           # SNR_ORTH_*
+MUON_NONE, MUON_SPECTRAL, MUON_RMS = 0, 1, 2          # SNR_MUON_*
+
 _NET, _RCFG = _c.POINTER(Net), _c.POINTER(RenderConfig)
 
 # name -> (restype, argtypes); mirrors include/spinnerf_hip.h one to one
@@ -123,6 +135,11 @@ SIGNATURES = {
     "snr_mse_pair": (_i, [_p, _p, _p, _l, _p, _p, _p, _p]),
     "snr_adam_step": (_i, [_p, _p, _p, _p, _l, _f, _f, _f, _f, _i, _f, _p]),
     "snr_adam_pack_multi": (_i, [_c.POINTER(AdamPackItem), _i, _f, _f, _f, _f, _i, _f, _p, _p]),
+    "snr_adam_step_multi": (_i, [_c.POINTER(AdamItem), _i, _f, _f, _f, _f, _i, _f, _p, _p]),
+    "snr_orthogonalise_ws_bytes": (_l, [_l, _l, _l, _i]),
+    "snr_orthogonalise": (_i, [_p, _i, _l, _l, _l, _l, _l, _p, _l, _l, _i, _f, _f, _f, _f, _i, _p, _p]),
+    "snr_muon_ws_bytes": (_l, [_c.POINTER(MuonItem), _i, _i]),
+    "snr_muon_step_multi": (_i, [_c.POINTER(MuonItem), _i, _f, _f, _i, _f, _i, _i, _f, _f, _f, _f, _f, _i, _p, _p, _p]),
     "snr_prof_enable": (_i, [_i]),
     "snr_prof_kernel_count": (_i, []),
     "snr_prof_kernel_name": (_c.c_char_p, [_i]),

@@ -23,6 +23,8 @@ SOURCES = [
     ("mlp_bwd.hip", ["-save-temps=obj"]),
     ("render_ops.hip", ["-ffp-contract=off"]),
     ("adam_pack.hip", ["-ffp-contract=off"]),    # Adam + weight pack in one kernel: must round like render_ops' adam_kernel
+    # no packed fp32 instructions: some of their forms have given wrong results on this card now and then
+    ("muon.hip", ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]),
     ("hashgrid.hip", ["-munsafe-fp-atomics"]),   # table gradients: hardware global_atomic_add_f32, no CAS loops
     ("prof.cpp", ["-x", "hip"]),
     ("fused.cpp", ["-x", "hip"]),                # render_rays as one call: launch order only, no kernels

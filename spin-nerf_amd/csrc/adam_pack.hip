@@ -225,6 +225,52 @@ __global__ __launch_bounds__(kApThreads) void adam_pack_kernel(AdamPackArgs a) {
   }
 }
 
+// ---- Adam on a list of ranges: the pieces of a flat buffer that another update does not cover ----------------------------
+constexpr int kAdamMulti = 48;   // ranges per launch: the kernel arguments hold the table
+constexpr int kAmThreads = 256, kAmBlock = 4 * kAmThreads;   // values per workgroup
+struct AdamRange { float* p; const float* g; float* m; float* v; int64_t n; int64_t block0; };
+struct AdamMultiArgs {
+  AdamRange r[kAdamMulti];
+  int n;
+  AdamCoef c;
+  const snr_step_state* st;
+};
+__global__ __launch_bounds__(kAmThreads) void adam_multi_kernel(AdamMultiArgs a) {
+  int s = 0;
+  while (s + 1 < a.n && (int64_t)blockIdx.x >= a.r[s + 1].block0) ++s;
+  const AdamRange& R = a.r[s];
+  AdamCoef c = a.c;
+  if (a.st) { c.lr = a.st->lr; c.bc1 = a.st->bc1; c.bc2_sqrt = a.st->bc2_sqrt; }
+  const int64_t i0 = ((int64_t)blockIdx.x - R.block0) * kAmBlock;
+  const bool wide = (((uintptr_t)R.p | (uintptr_t)R.g | (uintptr_t)R.m | (uintptr_t)R.v) & 15) == 0;
+  if (wide && i0 + kAmBlock <= R.n) {
+    const int64_t i = i0 + 4 * threadIdx.x;
+    f32x4 P = *(f32x4*)(R.p + i), M = *(f32x4*)(R.m + i), V = *(f32x4*)(R.v + i);
+    const f32x4 G = *(const f32x4*)(R.g + i);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float m = M[k], v = V[k];
+      P[k] = adam_one(P[k], G[k], m, v, c);
+      M[k] = m; V[k] = v;
+    }
+    *(f32x4*)(R.p + i) = P; *(f32x4*)(R.m + i) = M; *(f32x4*)(R.v + i) = V;
+    return;
+  }
+  // ranges off the 16-byte grid and tails: lanes side by side, every load ahead of the stores
+  float P[4], G[4], M[4], V[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int64_t i = i0 + threadIdx.x + kAmThreads * k;
+    const bool ok = i < R.n;
+    P[k] = ok ? R.p[i] : 0.f; G[k] = ok ? R.g[i] : 0.f; M[k] = ok ? R.m[i] : 0.f; V[k] = ok ? R.v[i] : 0.f;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int64_t i = i0 + threadIdx.x + kAmThreads * k;
+    if (i < R.n) { P[k] = adam_one(P[k], G[k], M[k], V[k], c); R.p[i] = P[k]; R.m[i] = M[k]; R.v[i] = V[k]; }
+  }
+}
+
 // beta^k by squaring, in double (render_ops.hip: powi — the same IEEE multiplications as the host side of snr_adam_step)
 static double powi_host(double b, long long k) {
   double r = 1.0;
@@ -300,4 +346,34 @@ extern "C" int snr_adam_pack_multi(const snr_adam_pack_item* items, int n_items,
     if (st != SNR_OK) return st;
   }
   return SNR_OK;
+}
+
+extern "C" int snr_adam_step_multi(const snr_adam_item* items, int n_items, float lr, float beta1, float beta2, float eps, int step,
+                                   float grad_scale, const snr_step_state* state, snr_stream_t stream) {
+  SNR_CHECK_ARG(items, SNR_ERR_NULL);
+  SNR_CHECK_ARG(n_items >= 1 && (state || step >= 1), SNR_ERR_SHAPE);
+  for (int i = 0; i < n_items; ++i) {
+    SNR_CHECK_ARG(items[i].n >= 0 && items[i].n <= (int64_t)1 << 40, SNR_ERR_SHAPE);
+    SNR_CHECK_ARG(items[i].n == 0 || (items[i].params && items[i].grads && items[i].exp_avg && items[i].exp_avg_sq), SNR_ERR_NULL);
+  }
+  const float bc1 = state ? 1.f : (float)(1.0 - powi_host((double)beta1, step));
+  const float bc2_sqrt = state ? 1.f : (float)sqrt(1.0 - powi_host((double)beta2, step));
+  for (int i = 0; i < n_items;) {
+    AdamMultiArgs a{};
+    int64_t blocks = 0;
+    for (; i < n_items && a.n < kAdamMulti; ++i) {
+      const snr_adam_item& it = items[i];
+      if (it.n == 0) continue;
+      const int64_t nb = (it.n + kAmBlock - 1) / kAmBlock;
+      if (blocks + nb > INT32_MAX) break;       // (the next launch takes it)
+      a.r[a.n++] = AdamRange{it.params, it.grads, it.exp_avg, it.exp_avg_sq, it.n, blocks};
+      blocks += nb;
+    }
+    if (!a.n) continue;
+    a.c = AdamCoef{lr, beta1, beta2, eps, bc1, bc2_sqrt, grad_scale};
+    a.st = state;
+    ProfScope ps(K_ADAM_MULTI, (hipStream_t)stream);
+    adam_multi_kernel<<<dim3((unsigned)blocks), dim3(kAmThreads), 0, (hipStream_t)stream>>>(a);
+  }
+  return launch_status();
 }

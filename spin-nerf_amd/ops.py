@@ -645,3 +645,180 @@ def adam_pack_step_(nets, grads, exp_avgs, exp_avg_sqs, lr, step, beta1=0.9, bet
     for net in nets:
         net.note_packed_in_place()
     return True
+
+
+def _flat_list(name, params, *others):
+    """the tensors of an in-place optimizer call as lists: fp32, contiguous, on one device, equal sizes item by item, and no two
+    of the tensors that are written sharing memory (the items of a launch run side by side)"""
+    lists = [list(params)] + [list(o) for o in others]
+    if any(len(x) != len(lists[0]) for x in lists):
+        raise ValueError(f"{name}: the lists differ in length: {[len(x) for x in lists]}")
+    dev = None
+    for row in zip(*lists):
+        for t in row:
+            if not t.is_cuda:
+                raise _lib.HipLibraryError(f"{name}: the kernels need device (HIP) tensors; got a CPU tensor")
+            dev = t.device if dev is None else dev
+            if t.device != dev:
+                raise ValueError(f"{name}: expected a tensor on {dev}, got {t.device}")
+            if t.dtype != torch.float32:
+                raise ValueError(f"{name}: expected float32, got {t.dtype}")
+            if t.shape != row[0].shape:
+                raise ValueError(f"{name}: shapes of one item differ: {[tuple(u.shape) for u in row]}")
+    return lists, dev
+
+
+def _no_overlap(name, read, written):
+    """no tensor of ``written`` shares memory with another of ``written`` or with one of ``read``"""
+    spans = sorted([(t.data_ptr(), t.data_ptr() + 4 * t.numel(), w) for ts, w in ((written, True), (read, False)) for t in ts if t.numel()])
+    end_w = end_any = 0
+    for a, b, w in spans:
+        if a < (end_any if w else end_w):
+            raise ValueError(f"{name}: a tensor that is written shares memory with another of the call")
+        end_any = max(end_any, b)
+        if w:
+            end_w = max(end_w, b)
+
+
+def _written(name, ts):
+    for t in ts:
+        if not t.is_contiguous():
+            raise ValueError(f"{name}: tensors that are written must be contiguous; got strides {t.stride()} for {tuple(t.shape)}")
+
+
+def adam_step_multi_(params, grads, exp_avgs, exp_avg_sqs, lr, step, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, state=None):
+    """adam_step_ (bit for bit) on lists of fp32 tensors of any sizes in one launch per 48 tensors (snr_adam_step_multi): what of a
+    network is no hidden matrix when muon_step_ takes the rest.  ``state``: a device-side snr_step_state whose rate and bias
+    corrections count instead of ``lr`` and ``step`` (captured graphs)."""
+    (params, grads, ms, vs), dev = _flat_list("adam_step_multi_", params, grads, exp_avgs, exp_avg_sqs)
+    if not params:
+        return
+    _written("adam_step_multi_", params + ms + vs)
+    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    _no_overlap("adam_step_multi_", grads, params + ms + vs)
+    lib = _lib.load()
+    items = (_lib.AdamItem * len(params))(*[(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel())
+                                            for p, g, m, v in zip(params, grads, ms, vs)])
+    with torch.cuda.device(dev):
+        check(lib.snr_adam_step_multi(items, len(params), float(lr), float(beta1), float(beta2), float(eps), int(step), float(grad_scale),
+                                      ptr(state), stream()), "snr_adam_step_multi")
+
+
+# ----------------------------------------------------------------------------------------------
+# orthogonalised updates: Newton-Schulz products, and the optimizer step around them
+# ----------------------------------------------------------------------------------------------
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)   # the quintic that lifts small singular values fastest and keeps them in [0.68, 1.13] or so
+_ORTH_TYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+_ORTH_PREC = {"fp16": _lib.ORTH_FP16, "fp32": _lib.ORTH_FP32}
+_MUON_SCALE = {"none": _lib.MUON_NONE, "spectral": _lib.MUON_SPECTRAL, "rms": _lib.MUON_RMS}
+
+
+def _orth_args(name, steps, coefficients, eps, precision):
+    if precision not in _ORTH_PREC:
+        raise ValueError(f"{name}: precision must be one of {sorted(_ORTH_PREC)}, got {precision!r}")
+    if int(steps) != steps or not 1 <= steps <= 100:
+        raise ValueError(f"{name}: steps must be a whole number from 1 to 100, got {steps!r}")
+    if not eps >= 1e-30:
+        raise ValueError(f"{name}: eps must be at least 1e-30, got {eps!r}")
+    a, b, c = (float(v) for v in coefficients)
+    return int(steps), a, b, c, float(eps), _ORTH_PREC[precision]
+
+
+def _orth_check(status, name, what):
+    if status == _lib.ERR_UNSUPPORTED:
+        raise ValueError(f"{name}: the coefficients must keep singular values from [0, 1] below 8 over all steps, and |b l + c l^2| "
+                         "below 64 for the squares l of all singular values on the way")
+    check(status, what)
+
+
+def orthogonalise(x, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, precision=None, out=None):
+    """x [..., m, n] with its singular values driven towards 1 and its singular vectors kept, in x's type:
+
+        X = x / max(|x|_F, eps);   steps times:  A = X X^T,  X <- a X + (b A + c A A) X        (a, b, c) = coefficients
+
+    ``precision``: "fp32" = every product at fp32's accuracy, "fp16" = products of fp16 roundings (2^-11) with fp32 sums, a third of
+    the matrix work (where the shorter side is above 64; below, it is "fp32"); default "fp16" for bf16 tensors (their own roundings are coarser) and "fp32" for the others.  A zero matrix
+    gives zeros, one with a NaN or an infinity NaN throughout.  ``out`` (contiguous, may be x): where the result goes.  Not
+    differentiable: an x that requires grad is refused unless grad mode is off."""
+    if not isinstance(x, torch.Tensor) or x.dim() < 2:
+        raise ValueError(f"orthogonalise: expected a tensor [..., m, n], got {tuple(x.shape) if isinstance(x, torch.Tensor) else type(x).__name__}")
+    if x.dtype not in _ORTH_TYPES:
+        raise ValueError(f"orthogonalise: expected float32, float16 or bfloat16, got {x.dtype}")
+    if torch.is_grad_enabled() and (x.requires_grad or (out is not None and out.requires_grad)):
+        raise RuntimeError("orthogonalise has no backward pass: call it under torch.no_grad() or on x.detach()")
+    args = _orth_args("orthogonalise", steps, coefficients, eps, precision or ("fp16" if x.dtype == torch.bfloat16 else "fp32"))
+    if not x.is_cuda:
+        raise _lib.HipLibraryError("orthogonalise: the kernels need device (HIP) tensors; got a CPU tensor")
+    if out is not None and (out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or not out.is_contiguous()):
+        raise ValueError("orthogonalise: out must be a contiguous tensor of x's shape, type and device")
+    # a transposed view is taken as it lies: its result is the transposed result
+    flip = x.stride(-1) != 1 and x.stride(-2) == 1 and x.shape[-1] > 1 and out is None
+    y = x.mT if flip else x
+    m, n = y.shape[-2:]
+    y = y.reshape(-1, m, n) if y.numel() else y
+    res = torch.empty(y.shape, device=x.device, dtype=x.dtype) if out is None else out
+    if y.numel():
+        if (n > 1 and y.stride(2) != 1) or (m > 1 and y.stride(1) < n):
+            y = y.contiguous()
+        elif out is not None and (y.data_ptr() != out.data_ptr() or not x.is_contiguous()) and _shares_memory(y, out):
+            y = y.clone()
+        lib = _lib.load()
+        dt, st, prec = _ORTH_TYPES[x.dtype], args[:5], args[5]
+        with torch.cuda.device(x.device):
+            nbytes = lib.snr_orthogonalise_ws_bytes(y.shape[0], m, n, prec)
+            if nbytes <= 0:
+                check(int(nbytes), "snr_orthogonalise_ws_bytes")
+            ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
+            _orth_check(lib.snr_orthogonalise(ptr(y), dt, y.shape[0], m, n, y.stride(0), max(y.stride(1), n), ptr(res), m * n, n, *st, prec,
+                                              ptr(ws), stream()), "orthogonalise", "snr_orthogonalise")
+    if out is not None:
+        return out
+    return res.reshape(x.mT.shape).mT if flip else res.reshape(x.shape)
+
+
+def _shares_memory(a, b):
+    """whether the spans of two tensors of one device touch (strided tensors by their whole span)"""
+    def span(t):
+        last = sum((s - 1) * st for s, st in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def muon_step_(params, grads, momentum_buffers, lr, momentum=0.95, nesterov=True, weight_decay=0.0, scale="spectral", steps=5,
+               coefficients=NEWTON_SCHULZ, eps=1e-7, grad_scale=1.0, precision="fp32", state=None):
+    """One optimizer step on hidden matrices, in place: lists of fp32 tensors [..., m, n] (leading dimensions: a stack of matrices).
+
+        momentum_buffer <- momentum * momentum_buffer + grad_scale * g
+        u = grad_scale * g + momentum * momentum_buffer   (nesterov), else momentum_buffer
+        p <- p (1 - lr weight_decay) - lr q orthogonalise(u)
+
+    ``scale``: q = sqrt(max(1, m / n)) ("spectral": a step moves every matrix's spectral norm by about lr), 0.2 sqrt(max(m, n))
+    ("rms": about the size of an Adam step at the same rate) or 1 ("none").  ``precision`` as in orthogonalise.  ``state``: a
+    device-side snr_step_state whose rate counts instead of ``lr`` (captured graphs).  Vectors, embeddings and output layers are
+    not meant here: adam_step_multi_ takes them."""
+    args = _orth_args("muon_step_", steps, coefficients, eps, precision)
+    if scale not in _MUON_SCALE:
+        raise ValueError(f"muon_step_: scale must be one of {sorted(_MUON_SCALE)}, got {scale!r}")
+    (params, grads, bufs), dev = _flat_list("muon_step_", params, grads, momentum_buffers)
+    if any(p.dim() < 2 for p in params):
+        raise ValueError(f"muon_step_: expected matrices [..., m, n], got {[tuple(p.shape) for p in params if p.dim() < 2][0]}")
+    live = [i for i, p in enumerate(params) if p.numel()]
+    if not live:
+        return
+    _written("muon_step_", params + bufs)
+    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    _no_overlap("muon_step_", grads, params + bufs)
+    lib = _lib.load()
+    items = (_lib.MuonItem * len(live))(*[(params[i].data_ptr(), grads[i].data_ptr(), bufs[i].data_ptr(),
+                                           params[i].numel() // (params[i].shape[-2] * params[i].shape[-1]), params[i].shape[-2],
+                                           params[i].shape[-1]) for i in live])
+    n_steps, a, b, c, eps, prec = args
+    with torch.cuda.device(dev):
+        nbytes = lib.snr_muon_ws_bytes(items, len(live), prec)
+        if nbytes <= 0:
+            check(int(nbytes), "snr_muon_ws_bytes")
+        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        _orth_check(lib.snr_muon_step_multi(items, len(live), float(lr), float(momentum), int(bool(nesterov)), float(weight_decay),
+                                            _MUON_SCALE[scale], n_steps, a, b, c, eps, float(grad_scale), prec, ptr(state), ptr(ws),
+                                            stream()), "muon_step_", "snr_muon_step_multi")
