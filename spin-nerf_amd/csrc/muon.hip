@@ -18,14 +18,13 @@
 namespace snr {
 
 constexpr int kOrthMax = 24;                // stacks per launch sequence: the kernel arguments hold the table
-constexpr int kTile = 64;                   // padding and output tile
+constexpr int kPad = 64;                    // what the planes' sides are padded to
 constexpr float kYs = 1024.f, kAs = 512.f;  // powers of two that the planes of Y and of A, B are scaled by
 constexpr float kLo = 2048.f;               // ... and the lo planes on top
 
 struct OrthGeom {        // a stack of equal matrices
   int r, c, rp, cp;      // sides of Y, and padded to the tile
-  int batch, split;      // split: the lo planes take part in the products
-  int sym0, full0;       // first workgroup of the stack in the symmetric products / in B Y
+  int batch;
   int64_t ws;            // its planes
 };
 struct OrthIo {
@@ -33,17 +32,19 @@ struct OrthIo {
   void* out;             // the result, or the parameters
   float* mom;            // momentum (null: plain orthogonalisation)
   int64_t xb, xr, ob, orow;  // element strides: matrix, row (columns are contiguous)
-  int m, n, chunk0, split0;  // sizes as stored; first workgroup in the reduction / in the split
+  int m, n;              // sizes as stored
   int nchunk;            // workgroups (partial sums) per matrix in the reduction
   int64_t part;          // first partial sum (doubles)
 };
 struct OrthTable { int n; OrthGeom g[kOrthMax]; };
-struct OrthArgs {
+struct OrthArgs {        // kernel arguments: a miss on them costs a microsecond, so the stack is found by one load (find_stack)
+  int sym0[kOrthMax], full0[kOrthMax], chunk0[kOrthMax], split0[kOrthMax];   // each stack's first workgroup: symmetric products, B Y,
+                                                                             // reduction, split
   OrthTable t;
   OrthIo io[kOrthMax];
   int dtype;             // of x / out without momentum
   float mu, gscale, eps;
-  int nesterov;
+  int nesterov, split;
   double* part;
   char* ws;
 };
@@ -53,14 +54,24 @@ struct OrthOut {         // the last product's epilogue
   const snr_step_state* st;
 };
 
-// planes of one matrix, in fp16 elements
-struct OrthPlanes { int64_t yh, yl, t0h, t0l, t1h, t1l, ah, al, bh, bl, total; };
-__host__ __device__ inline OrthPlanes orth_planes(int rp, int cp) {
+// Planes of one matrix, in fp16 elements.  Y has two places, a step reads one and writes the other.  Without the split products the
+// lo planes of A and B do not exist (B = b A + c A^2 takes A's rounding in both terms: near s = 1 the two errors cancel in part), and
+// Y's lo plane, which only the workgroup of its own tile reads then, has one place.
+struct OrthPlanes { int64_t h[2], l[2], ah, al, bh, bl, total; };
+__host__ __device__ inline OrthPlanes orth_planes(int rp, int cp, bool split) {
   const int64_t y = (int64_t)rp * cp, g = (int64_t)rp * rp;
   OrthPlanes p;
-  p.yh = 0; p.yl = y; p.t0h = 2 * y; p.t0l = 3 * y; p.t1h = 4 * y; p.t1l = 5 * y;
-  p.ah = 6 * y; p.al = p.ah + g; p.bh = p.al + g; p.bl = p.bh + g; p.total = p.bl + g;
+  p.h[0] = 0; p.h[1] = y; p.l[0] = 2 * y; p.l[1] = split ? 3 * y : 2 * y;
+  p.ah = p.l[1] + y; p.bh = p.ah + g; p.al = p.bh + (split ? g : 0); p.bl = p.al + (split ? g : 0);
+  p.total = (split ? p.bl : p.bh) + g;
   return p;
+}
+
+// the stack a workgroup belongs to: its lanes look at every stack's first workgroup at once
+__device__ __forceinline__ int find_stack(const int* first, int n, int block) {
+  const int lane = threadIdx.x & 63;
+  const bool mine = lane < n && block >= first[lane < n ? lane : 0];
+  return __builtin_amdgcn_readfirstlane(__popcll(__ballot(mine)) - 1);
 }
 
 __device__ __forceinline__ float orth_load(const void* p, int64_t i, int dtype) {
@@ -80,10 +91,9 @@ __device__ __forceinline__ void orth_split(float v, _Float16& hi, _Float16& lo) 
 
 // ---- 1. momentum (in place) and the partial sums of squares of the update, in 64 bits and in a fixed order ------------------
 __global__ __launch_bounds__(256) void orth_reduce_kernel(OrthArgs a) {
-  int s = 0;
-  while (s + 1 < a.t.n && (int)blockIdx.x >= a.io[s + 1].chunk0) ++s;
+  const int s = find_stack(a.chunk0, a.t.n, blockIdx.x);
   const OrthIo& io = a.io[s];
-  const int k = blockIdx.x - io.chunk0, mat = k / io.nchunk, ch = k % io.nchunk;
+  const int k = blockIdx.x - a.chunk0[s], mat = k / io.nchunk, ch = k % io.nchunk;
   const int64_t count = (int64_t)io.m * io.n;
   const int64_t per = (count + io.nchunk - 1) / io.nchunk, e0 = ch * per, e1 = e0 + per < count ? e0 + per : count;
   double sum = 0.0;
@@ -109,18 +119,17 @@ __global__ __launch_bounds__(256) void orth_reduce_kernel(OrthArgs a) {
   if (threadIdx.x == 0) a.part[io.part + mat * io.nchunk + ch] = red[0];
 }
 
-// ---- 2. Y = scaled input (transposed where it is tall) and Y^T, as planes, zero in the padding --------------------------------
+// ---- 2. Y = scaled input (transposed where it is tall) as planes, zero in the padding --------------------------------------------
 __global__ __launch_bounds__(256) void orth_split_kernel(OrthArgs a) {
-  int s = 0;
-  while (s + 1 < a.t.n && (int)blockIdx.x >= a.io[s + 1].split0) ++s;
+  const int s = find_stack(a.split0, a.t.n, blockIdx.x);
   const OrthIo& io = a.io[s];
   const OrthGeom& G = a.t.g[s];
-  const int nti = G.rp / kTile, ntj = G.cp / kTile;
-  const int k = blockIdx.x - io.split0, mat = k / (nti * ntj), t = k % (nti * ntj);
-  const int i0 = t / ntj * kTile, j0 = t % ntj * kTile;
+  const int nti = G.rp / kPad, ntj = G.cp / kPad;
+  const int k = blockIdx.x - a.split0[s], mat = k / (nti * ntj), t = k % (nti * ntj);
+  const int i0 = t / ntj * kPad, j0 = t % ntj * kPad;
   const bool tall = io.m > io.n;
   __shared__ double red[256];
-  __shared__ float tile[kTile][kTile + 1];
+  __shared__ float tile[kPad][kPad + 1];
   double sum = 0.0;
   for (int p = threadIdx.x; p < io.nchunk; p += 256) sum += a.part[io.part + mat * io.nchunk + p];
   red[threadIdx.x] = sum;
@@ -133,7 +142,7 @@ __global__ __launch_bounds__(256) void orth_split_kernel(OrthArgs a) {
   const double scale = (double)kYs / (norm < (double)a.eps ? (double)a.eps : norm);   // (a NaN stays one)
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   // rows of the input are contiguous: lanes run along them
-  for (int q = w; q < kTile; q += 4) {
+  for (int q = w; q < kPad; q += 4) {
     const int mi = tall ? j0 + q : i0 + q, nj = (tall ? i0 : j0) + lane;
     float u = 0.f;
     if (mi < io.m && nj < io.n) {
@@ -149,83 +158,254 @@ __global__ __launch_bounds__(256) void orth_split_kernel(OrthArgs a) {
     if (tall) tile[lane][q] = u; else tile[q][lane] = u;
   }
   __syncthreads();
-  const OrthPlanes P = orth_planes(G.rp, G.cp);
+  const OrthPlanes P = orth_planes(G.rp, G.cp, a.split);
   _Float16* W = (_Float16*)(a.ws + G.ws) + mat * P.total;
-  for (int q = w; q < kTile; q += 4) {
+  for (int q = w; q < kPad; q += 4) {
     _Float16 hi, lo;
     orth_split(tile[q][lane], hi, lo);
     const int64_t y = (int64_t)(i0 + q) * G.cp + j0 + lane;
-    W[P.yh + y] = hi; W[P.yl + y] = lo;
-    orth_split(tile[lane][q], hi, lo);
-    const int64_t yt = (int64_t)(j0 + q) * G.rp + i0 + lane;
-    W[P.t0h + yt] = hi; W[P.t0l + yt] = lo;
+    W[P.h[0] + y] = hi; W[P.l[0] + y] = lo;
   }
 }
 
-// ---- 3. the products: C[i][j] = sum_k P[i][k] Q[j][k], rows contiguous in k ----------------------------------------------------
-//   phase 0: A = Y Y^T          (symmetric: tiles i <= j, mirrored)
-//   phase 1: B = b A + c A A^T  (symmetric)
-//   phase 2: Y <- a Y + B Y, taken as B (Y^T)^T; also Y^T for the next step, or the result
-enum { kGram = 0, kPoly = 1, kApply = 2 };
-constexpr int kLd = kTile + 8;   // LDS row of 64 + 8 fp16: 144 B, 16-byte reads of 32 rows spread over the banks
+// ---- 3. the products -------------------------------------------------------------------------------------------------------------
+//   Gram:  A = Y Y^T          (symmetric: tiles i <= j, mirrored)
+//   Poly:  B = b A + c A A^T  (symmetric)
+//   Apply: Y <- a Y + B Y, or the result
+//
+// A workgroup makes a T x T tile C[i][j] = sum_k P[i][k] Q[j][k] (Apply: Q[k][j]) from BK-wide slices of K that stream through LDS by DMA
+// (16 B a lane), STAGES - 1 of them in flight.  A slice's rows of P are RB bytes, their 16 B chunks permuted so that the 16 rows that
+// 16 lanes read at one k fall on different banks; Apply's Q slice has rows of T columns, read transposed (ds_read_b64_tr_b16: four k of
+// a column to a lane).  The planes are padded to 64 only: a tile that hangs over reads the last row or column again and drops what
+// comes of it.
+enum { kGram = 0, kPoly = 1, kApply = 2 };   // template PHASE; LAST: the result instead of planes
 
-template <int PHASE>
-__global__ __launch_bounds__(256) void orth_product_kernel(OrthArgs a, OrthOut o, float ca, float cb, float cc, int flip, int last) {
-  int s = 0;
-  if (PHASE == kApply) { while (s + 1 < a.t.n && (int)blockIdx.x >= a.t.g[s + 1].full0) ++s; }
-  else { while (s + 1 < a.t.n && (int)blockIdx.x >= a.t.g[s + 1].sym0) ++s; }
+template <int T_, int WI_, int WJ_, bool SPLIT_, int STAGES_, int BK_> struct TileCfg {
+  static constexpr int BAND = T_ >= 192 ? 4 : 8;                  // tiles side by side that an XCD takes together
+  static constexpr int BK = BK_, CH = BK_ / 8, RB = 2 * BK_, RPL = 1024 / RB, STAGES = STAGES_, T = T_, WI = WI_, WJ = WJ_, NW = WI_ * WJ_, NT = 64 * NW;
+  static constexpr bool SPLIT = SPLIT_;
+  static constexpr int TI = T / WI / 32, TJ = T / WJ / 32;       // 32 x 32 blocks of a wave
+  static constexpr int SECT = T * RB;                             // bytes of one operand plane's slice
+  static constexpr int STAGE = SECT * (SPLIT ? 4 : 2);
+  static constexpr int PER = T / RPL / NW;                        // DMA instructions of a wave per plane: RPL rows each
+  static_assert(T % (RPL * NW) == 0 && T % (32 * WI) == 0 && T % (32 * WJ) == 0, "whole blocks");
+  static constexpr int LOADS = PER * (SPLIT ? 4 : 2);             // ... per slice
+  // where 16-byte chunk c of row r lies in a slice's plane
+  static __host__ __device__ constexpr int swz(int r, int c) { return r * RB + ((c ^ (BK == 64 ? (r >> 1) & 7 : (r >> 2) & 3)) << 4); }
+  // ... and, in Apply's Q slice, chunk c of row k: the 64 B that a group of 16 lanes reads of four rows fall on different banks
+  static __host__ __device__ constexpr int swzt(int k, int c) { return k * 2 * T + ((c ^ (T % 128 == 0 ? (k & 3) << 2 : (k >> 1 & 1) << 2)) << 4); }
+  static constexpr int EPI = NW * 32 * 36 * 4;                    // epilogue: a 32 x 36 fp32 block a wave
+};
+
+// 16 bytes a lane from base + off straight to LDS at dst + 16 lane.  In asm, as the compiler cannot tell which LDS reads such a load
+// concerns and waits for all of them; the waits are landed()'s.  It has no register to be overwritten, and it is counted in order
+// with every other load, so that the compiler's own waits only get stricter.
+__device__ __forceinline__ void dma16(unsigned dst, const _Float16* base, unsigned off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ unsigned lds_at(const char* p) { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p; }
+
+// a slice past the end is one 16-byte piece again and again: the number of loads in flight stays what the waits count on
+template <class C>
+__device__ __forceinline__ void fetch_slice(unsigned dst, const _Float16* const (&src)[4], const unsigned (&voff)[2][C::PER], int k, int n, int64_t ldq, int wave) {
+  const int k0 = k < n ? k * C::BK : 0;
+  const unsigned keep = k < n ? ~0u : 0u;
+#pragma unroll
+  for (int p = 0; p < (C::SPLIT ? 4 : 2); ++p) {
+    const _Float16* base = src[p] + (p & 1 ? k0 * ldq : k0);
+#pragma unroll
+    for (int q = 0; q < C::PER; ++q) dma16(dst + p * C::SECT + (wave + q * C::NW) * 1024, base, voff[p & 1][q] & keep);
+  }
+}
+
+// one slice: the fragments of the next 16 of K are read while those of this 16 are multiplied (sched_barrier keeps the compiler from
+// moving the reads back to their use: a wave alone on its SIMD would wait out LDS's latency eight times a slice)
+template <class C> struct Frags { f16x8 x[C::TI], y[C::TJ], xl[C::SPLIT ? C::TI : 1], yl[C::SPLIT ? C::TJ : 1]; };
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+// eight k of 32 columns from rows of columns: lane l gets column l % 32, k = 8 (l / 32) + 0 .. 7 of the 16 at kk; of a group of 16 lanes
+// lane i points at four columns of row i / 4, and receives one column of the four rows
+template <class C> __device__ __forceinline__ f16x8 read_turned(const char* src, int kk, int col, int lane) {
+  const int k = 16 * kk + 8 * (lane >> 5) + ((lane & 15) >> 2), c = col + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
+  auto part = [&](int kq) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(src + C::swzt(kq, c >> 3) + (c & 4) * 2)); };
+  union { s16x4 q[2]; f16x8 v; } u;
+  u.q[0] = part(k); u.q[1] = part(k + 4);
+  return u.v;
+}
+template <class C, bool TURN> __device__ __forceinline__ void read_frags(Frags<C>& f, const char* src, int kk, int wi, int wj, int lane) {
+  const int at = C::swz(lane & 31, 2 * kk + (lane >> 5));
+#pragma unroll
+  for (int i = 0; i < C::TI; ++i) f.x[i] = *(const f16x8*)(src + (wi + 32 * i) * C::RB + at);
+#pragma unroll
+  for (int j = 0; j < C::TJ; ++j) {
+    if constexpr (TURN) f.y[j] = read_turned<C>(src + C::SECT, kk, wj + 32 * j, lane);
+    else f.y[j] = *(const f16x8*)(src + C::SECT + (wj + 32 * j) * C::RB + at);
+  }
+  if constexpr (C::SPLIT) {
+#pragma unroll
+    for (int i = 0; i < C::TI; ++i) f.xl[i] = *(const f16x8*)(src + 2 * C::SECT + (wi + 32 * i) * C::RB + at);
+#pragma unroll
+    for (int j = 0; j < C::TJ; ++j) {
+      if constexpr (TURN) f.yl[j] = read_turned<C>(src + 3 * C::SECT, kk, wj + 32 * j, lane);
+      else f.yl[j] = *(const f16x8*)(src + 3 * C::SECT + (wj + 32 * j) * C::RB + at);
+    }
+  }
+}
+template <class C>
+__device__ __forceinline__ void mul_frags(const Frags<C>& g, f32x16 (&acc)[C::TI][C::TJ], f32x16 (&acl)[C::SPLIT ? C::TI : 1][C::SPLIT ? C::TJ : 1]) {
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < C::TI; ++i)
+#pragma unroll
+    for (int j = 0; j < C::TJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(g.x[i], g.y[j], acc[i][j], 0, 0, 0);
+  if constexpr (C::SPLIT) {
+#pragma unroll
+    for (int i = 0; i < C::TI; ++i)
+#pragma unroll
+      for (int j = 0; j < C::TJ; ++j) acl[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(g.x[i], g.yl[j], acl[i][j], 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < C::TI; ++i)
+#pragma unroll
+      for (int j = 0; j < C::TJ; ++j) acl[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(g.xl[i], g.y[j], acl[i][j], 0, 0, 0);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// this wave's DMA has landed but for the last N loads, and its LDS reads are done; then every wave's
+template <int N> __device__ __forceinline__ void landed() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4 << 14));   // vmcnt(N) lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// what lanes of this wave wrote to LDS is read by others of it
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// 16 consecutive fp16 of a row (32 B) as two vectors
+struct Half16 { f16x8 a, b; };
+__device__ __forceinline__ Half16 load16(const _Float16* p) { return Half16{*(const f16x8*)p, *(const f16x8*)(p + 8)}; }
+template <bool LO> __device__ __forceinline__ void store16(const float (&v)[16], _Float16* hi, _Float16* lo) {
+  f16x8 h[2], l[2];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    _Float16 a, b;
+    orth_split(v[e], a, b);
+    h[e >> 3][e & 7] = a; l[e >> 3][e & 7] = b;
+  }
+  *(f16x8*)hi = h[0]; *(f16x8*)(hi + 8) = h[1];
+  if constexpr (LO) { *(f16x8*)lo = l[0]; *(f16x8*)(lo + 8) = l[1]; }
+}
+
+// Workgroups go round the 8 XCDs, each with its own L2: number them so that an XCD has a run of neighbours, which share operand rows.
+__device__ __forceinline__ int xcd_block() {
+  const int n = gridDim.x, q = n >> 3, rem = n & 7, x = blockIdx.x & 7;
+  return x * q + (x < rem ? x : rem) + (blockIdx.x >> 3);
+}
+// tile t of the upper triangle (ti <= tj) of n x n tiles, taken in bands of BAND columns, row by row within a band
+template <int BAND> __device__ __forceinline__ void sym_tile(int t, int n, int& ti, int& tj) {
+  int b = (int)((sqrtf(8.f * t + 1.f) - 1.f) * (0.5f / BAND));     // column c starts at tile c (c + 1) / 2
+  while (b > 0 && BAND * b * (BAND * b + 1) / 2 > t) --b;
+  while (BAND * (b + 1) < n && BAND * (b + 1) * (BAND * (b + 1) + 1) / 2 <= t) ++b;
+  const int c0 = BAND * b, w = n - c0 < BAND ? n - c0 : BAND;
+  int q = t - c0 * (c0 + 1) / 2;
+  if (q < (c0 + 1) * w) { ti = q / w; tj = c0 + q % w; return; }
+  q -= (c0 + 1) * w;
+  int r = 1;
+  while (q >= w - r) { q -= w - r; ++r; }
+  ti = c0 + r; tj = c0 + r + q;
+}
+
+template <int PHASE, bool last, class C>
+__global__ __launch_bounds__(C::NT) void orth_product_kernel(OrthArgs a, OrthOut o, float ca, float cb, float cc, int flip) {
+  // one array per stage: the compiler tells a DMA into one from a read of another by the object
+  __shared__ __attribute__((aligned(16))) char s0[C::STAGE > C::EPI ? C::STAGE : C::EPI];
+  __shared__ __attribute__((aligned(16))) char s1[C::STAGE];
+  __shared__ __attribute__((aligned(16))) char s2[C::STAGES > 2 ? C::STAGE : 16];
+  __shared__ __attribute__((aligned(16))) char s3[C::STAGES > 3 ? C::STAGE : 16];
+  char* const buf[4] = {s0, s1, s2, s3};
+  const unsigned at[4] = {lds_at(s0), lds_at(s1), lds_at(s2), lds_at(s3)};
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int block = xcd_block();
+  const int s = find_stack(PHASE == kApply ? a.full0 : a.sym0, a.t.n, block);
   const OrthGeom& G = a.t.g[s];
-  const int nti = G.rp / kTile;
+  const int nti = (G.rp + C::T - 1) / C::T;
   int mat, ti, tj;
   if (PHASE == kApply) {
-    const int ntj = G.cp / kTile, k = blockIdx.x - G.full0;
-    mat = k / (nti * ntj); ti = k % (nti * ntj) / ntj; tj = k % ntj;
+    const int ntj = (G.cp + C::T - 1) / C::T, k = block - a.full0[s], t = k % (nti * ntj), band = t / (C::BAND * ntj);
+    const int h = nti - band * C::BAND < C::BAND ? nti - band * C::BAND : C::BAND, q = t - band * C::BAND * ntj;
+    mat = k / (nti * ntj); ti = band * C::BAND + q % h; tj = q / h;
   } else {
-    const int per = nti * (nti + 1) / 2, k = blockIdx.x - G.sym0;
-    mat = k / per; tj = 0;
-    int t = k % per;                       // column tj holds tj + 1 tiles
-    while (t > tj) { t -= tj + 1; ++tj; }
-    ti = t;
+    const int per = nti * (nti + 1) / 2, k = block - a.sym0[s];
+    mat = k / per;
+    sym_tile<C::BAND>(k % per, nti, ti, tj);
   }
-  const OrthPlanes P = orth_planes(G.rp, G.cp);
+  const OrthPlanes P = orth_planes(G.rp, G.cp, C::SPLIT);
   _Float16* W = (_Float16*)(a.ws + G.ws) + mat * P.total;
-  const int64_t th = flip ? P.t1h : P.t0h, tl = flip ? P.t1l : P.t0l;
-  const _Float16* ph = W + (PHASE == kGram ? P.yh : PHASE == kPoly ? P.ah : P.bh);
-  const _Float16* pl = W + (PHASE == kGram ? P.yl : PHASE == kPoly ? P.al : P.bl);
-  const _Float16* qh = W + (PHASE == kGram ? P.yh : PHASE == kPoly ? P.ah : th);
-  const _Float16* ql = W + (PHASE == kGram ? P.yl : PHASE == kPoly ? P.al : tl);
-  const int ld = PHASE == kGram ? G.cp : G.rp, K = ld;
-  constexpr int NP = 4;
-  const bool split = G.split;
-  __shared__ _Float16 lds[NP][kTile * kLd];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
-  f32x16 acc = {}, acl = {};
-  const _Float16* src[4] = {ph + (int64_t)ti * kTile * ld, qh + (int64_t)tj * kTile * ld, pl + (int64_t)ti * kTile * ld,
-                            ql + (int64_t)tj * kTile * ld};
-  for (int k0 = 0; k0 < K; k0 += kTile) {
+  const int64_t yh = flip ? P.h[1] : P.h[0], yl = flip ? P.l[1] : P.l[0];
+  const int K = PHASE == kGram ? G.cp : G.rp;
+  const int64_t ldq = PHASE == kApply ? G.cp : 1;      // how far apart slices of Q lie, an element of k
+  const int64_t ph = PHASE == kGram ? yh : PHASE == kPoly ? P.ah : P.bh, pl = PHASE == kGram ? yl : PHASE == kPoly ? P.al : P.bl;
+  const int64_t pi = (int64_t)ti * C::T * K, qj = PHASE == kApply ? (int64_t)tj * C::T : (int64_t)tj * C::T * K;
+  const _Float16* src[4] = {W + ph + pi, W + (PHASE == kApply ? yh : ph) + qj, W + pl + pi, W + (PHASE == kApply ? yl : pl) + qj};
+  unsigned voff[2][C::PER];         // bytes
 #pragma unroll
-    for (int p = 0; p < NP; ++p)
+  for (int q = 0; q < C::PER; ++q) {
+    const int blk = wave + q * C::NW, row = blk * C::RPL + lane / C::CH, col = (C::swz(row, lane % C::CH) - row * C::RB) / 2;
+    const int lp = G.rp - 1 - ti * C::T;
+    voff[0][q] = 2u * ((row < lp ? row : lp) * K + col);
+    if constexpr (PHASE == kApply) {
+      const int at = blk * 64 + lane, kr = at / (C::T / 8), kc = (C::swzt(kr, at % (C::T / 8)) - kr * 2 * C::T) / 2, lc = G.cp - 8 - tj * C::T;
+      voff[1][q] = 2u * (kr * G.cp + (kc < lc ? kc : lc));
+    } else {
+      const int lq = G.rp - 1 - tj * C::T;
+      voff[1][q] = 2u * ((row < lq ? row : lq) * K + col);
+    }
+  }
+  const int wi = (wave / C::WJ) * (C::T / C::WI), wj = (wave % C::WJ) * (C::T / C::WJ);
+  f32x16 acc[C::TI][C::TJ] = {}, acl[C::SPLIT ? C::TI : 1][C::SPLIT ? C::TJ : 1] = {};
+  const int n = K / C::BK;
+  // Slice k's last 16 of K are multiplied behind the barrier that frees its buffer and shows slice k + 1, whose first fragments are
+  // read under them; slice k + STAGES is fetched into the buffer at once.
+  constexpr int KK = C::BK / 16;
+  Frags<C> f[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (p >= 2 && !split) continue;
-        const int ck = tid + 256 * h, row = ck >> 3, col = (ck & 7) * 8;
-        *(f16x8*)&lds[p][row * kLd + col] = *(const f16x8*)(src[p] + (int64_t)row * ld + k0 + col);
-      }
-    __syncthreads();
+  for (int u = 0; u < C::STAGES; ++u) fetch_slice<C>(at[u], src, voff, u, n, ldq, wave);
+  landed<(C::STAGES - 1) * C::LOADS>();
+  read_frags<C, PHASE == kApply>(f[0], s0, 0, wi, wj, lane);
+  int k = 0;
+  for (; k + C::STAGES <= n; k += C::STAGES) {
 #pragma unroll
-    for (int kk = 0; kk < kTile; kk += 16) {
-      const int at = (lane & 31) * kLd + kk + 8 * (lane >> 5);
-      const f16x8 x = *(const f16x8*)&lds[0][wi * kLd + at], y = *(const f16x8*)&lds[1][wj * kLd + at];
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, acc, 0, 0, 0);
-      if (split) {
-        const f16x8 xl = *(const f16x8*)&lds[NP - 2][wi * kLd + at], yl = *(const f16x8*)&lds[NP - 1][wj * kLd + at];
-        acl = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, yl, acl, 0, 0, 0);
-        acl = __builtin_amdgcn_mfma_f32_32x32x16_f16(xl, y, acl, 0, 0, 0);
+    for (int u = 0; u < C::STAGES; ++u) {
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        if (kk + 1 < KK) read_frags<C, PHASE == kApply>(f[(kk + 1) & 1], buf[u], kk + 1, wi, wj, lane);
+        else {
+          landed<(C::STAGES - 2) * C::LOADS>();
+          fetch_slice<C>(at[u], src, voff, k + u + C::STAGES, n, ldq, wave);
+          read_frags<C, PHASE == kApply>(f[0], buf[(u + 1) % C::STAGES], 0, wi, wj, lane);
+        }
+        mul_frags<C>(f[kk & 1], acc, acl);
       }
     }
-    __syncthreads();
   }
+  landed<0>();
+#pragma unroll
+  for (int u = 0; u < C::STAGES - 1; ++u)
+    if (k + u < n) {
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        if (u || kk) read_frags<C, PHASE == kApply>(f[kk & 1], buf[u], kk, wi, wj, lane);
+        mul_frags<C>(f[kk & 1], acc, acl);
+      }
+    }
+  landed<0>();
+
+  // epilogue: a wave turns its 32 x 32 blocks in LDS, so that rows (and, for the mirrored or transposed copy, columns) are written
+  // 32 B a lane
+  float (*blk)[36] = (float (*)[36])(s0 + wave * (32 * 36 * 4));
   float lr_q = 0.f, keep = 1.f;
   if (PHASE == kApply && last && o.muon) {
     const float lr = o.st ? o.st->lr : o.lr;
@@ -233,37 +413,64 @@ __global__ __launch_bounds__(256) void orth_product_kernel(OrthArgs a, OrthOut o
     const float q = o.scale_mode == SNR_MUON_SPECTRAL ? sqrtf(fmaxf(1.f, m / n)) : o.scale_mode == SNR_MUON_RMS ? 0.2f * sqrtf(fmaxf(m, n)) : 1.f;
     lr_q = lr * q; keep = 1.f - lr * o.decay;
   }
-  const int j = tj * kTile + wj + (lane & 31);
+  const int row = lane >> 1, c0 = (lane & 1) * 16;
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const int i = ti * kTile + wi + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-    float v = acc[e] + acl[e] * (1.f / kLo);
-    _Float16 hi, lo;
-    if (PHASE == kGram || PHASE == kPoly) {
-      if (PHASE == kGram) v *= kAs / (kYs * kYs);
-      else v = cb * ((float)W[P.ah + (int64_t)i * G.rp + j] + (float)W[P.al + (int64_t)i * G.rp + j] * (1.f / kLo)) + cc * (v * (1.f / kAs));
-      orth_split(v, hi, lo);
-      const int64_t dh = PHASE == kGram ? P.ah : P.bh, dl = PHASE == kGram ? P.al : P.bl;
-      W[dh + (int64_t)i * G.rp + j] = hi; W[dl + (int64_t)i * G.rp + j] = lo;
-      if (ti != tj) { W[dh + (int64_t)j * G.rp + i] = hi; W[dl + (int64_t)j * G.rp + i] = lo; }
-    } else {
-      const int64_t y = (int64_t)i * G.cp + j;
-      v = ca * ((float)W[P.yh + y] + (float)W[P.yl + y] * (1.f / kLo)) + v * (1.f / kAs);
-      if (!last) {
-        orth_split(v, hi, lo);
-        W[P.yh + y] = hi; W[P.yl + y] = lo;
-        const int64_t yt = (int64_t)j * G.rp + i, nh = flip ? P.t0h : P.t1h, nl = flip ? P.t0l : P.t1l;
-        W[nh + yt] = hi; W[nl + yt] = lo;
-      } else if (i < G.r && j < G.c) {
+  for (int bi = 0; bi < C::TI; ++bi)
+#pragma unroll
+    for (int bj = 0; bj < C::TJ; ++bj) {
+      const int i0 = ti * C::T + wi + 32 * bi, j0 = tj * C::T + wj + 32 * bj;
+      if (i0 >= G.rp || j0 >= (PHASE == kApply ? G.cp : G.rp)) continue;
+      wave_sync();
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        float v = acc[bi][bj][e];
+        if constexpr (C::SPLIT) v += acl[bi][bj][e] * (1.f / kLo);
+        blk[8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)][lane & 31] = v;
+      }
+      wave_sync();
+      float v[16];
+      const int64_t y = (int64_t)(i0 + row) * (PHASE == kApply ? G.cp : G.rp) + j0 + c0;
+      if (PHASE == kGram) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = blk[row][c0 + e] * (kAs / (kYs * kYs));
+      } else {
+        const Half16 h = load16(W + (PHASE == kPoly ? P.ah : yh) + y);
+        Half16 l;
+        if (PHASE == kApply || C::SPLIT) l = load16(W + (PHASE == kPoly ? P.al : yl) + y);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float old = (float)(e < 8 ? h.a[e & 7] : h.b[e & 7]);
+          if (PHASE == kApply || C::SPLIT) old += (float)(e < 8 ? l.a[e & 7] : l.b[e & 7]) * (1.f / kLo);
+          v[e] = PHASE == kPoly ? cb * old + cc * (blk[row][c0 + e] * (1.f / kAs)) : ca * old + blk[row][c0 + e] * (1.f / kAs);
+        }
+      }
+      const int64_t dh = PHASE == kGram ? P.ah : PHASE == kPoly ? P.bh : flip ? P.h[0] : P.h[1];
+      const int64_t dl = PHASE == kGram ? P.al : PHASE == kPoly ? P.bl : flip ? P.l[0] : P.l[1];
+      if (!last) store16<PHASE == kApply || C::SPLIT>(v, W + dh + y, W + dl + y);
+      if (PHASE == kApply ? !last : ti == tj) continue;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) blk[row][c0 + e] = v[e];
+      wave_sync();
+      if (PHASE != kApply) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = blk[c0 + e][row];
+        const int64_t yt = (int64_t)(j0 + row) * G.rp + i0 + c0;
+        store16<C::SPLIT>(v, W + dh + yt, W + dl + yt);
+      } else {
         const OrthIo& io = a.io[s];
         const bool tall = io.m > io.n;
-        const int64_t at = mat * io.ob + (tall ? (int64_t)j * io.orow + i : (int64_t)i * io.orow + j);
-        v *= 1.f / kYs;
-        if (o.muon) { float* p = (float*)io.out + at; *p = *p * keep - lr_q * v; }
-        else orth_store(io.out, at, o.dtype, v);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int u = 2 * e + (lane >> 5), w = lane & 31;       // lanes along the result's rows
+          const int i = i0 + (tall ? w : u), j = j0 + (tall ? u : w);
+          if (i >= G.r || j >= G.c) continue;
+          const float x = (tall ? blk[w][u] : blk[u][w]) * (1.f / kYs);
+          const int64_t at = mat * io.ob + (tall ? (int64_t)j * io.orow + i : (int64_t)i * io.orow + j);
+          if (o.muon) { float* p = (float*)io.out + at; *p = *p * keep - lr_q * x; }
+          else orth_store(io.out, at, o.dtype, x);
+        }
       }
     }
-  }
 }
 
 }  // namespace snr
@@ -299,27 +506,55 @@ static bool orth_bounded(int steps, double a, double b, double c) {
   return true;
 }
 
+#ifndef NS64
+#define NS64 4
+#define NH64 4
+#define NH128 2
+#define BK128 64
+#define NH256 2
+#define BK256 64
+#endif
 static int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 static int orth_chunks(int64_t count) {
   const int64_t n = (count + 4095) / 4096;
   return (int)(n < 1 ? 1 : n > 1024 ? 1024 : n);
 }
-static int64_t matrix_bytes(int64_t m, int64_t n) {
+static int64_t matrix_bytes(int64_t m, int64_t n, bool split) {
   const int64_t r = m < n ? m : n, c = m < n ? n : m;
-  return align256(orth_planes((int)((r + kTile - 1) / kTile * kTile), (int)((c + kTile - 1) / kTile * kTile)).total * 2);
+  return align256(orth_planes((int)((r + kPad - 1) / kPad * kPad), (int)((c + kPad - 1) / kPad * kPad), split).total * 2);
 }
 static const int64_t kMaxSide = 65536, kMaxBatch = 65536;
 static int stack_ok(int64_t batch, int64_t m, int64_t n) {
   if (batch < 1 || m < 1 || n < 1 || m > kMaxSide || n > kMaxSide || batch > kMaxBatch) return SNR_ERR_SHAPE;
   return SNR_OK;
 }
-static int64_t stack_bytes(int64_t batch, int64_t m, int64_t n) {
-  return align256(batch * orth_chunks(m * n) * 8) + batch * matrix_bytes(m, n);
+static bool splits(int precision, int64_t m, int64_t n) { return precision == SNR_ORTH_FP32 || m <= 64 || n <= 64; }
+static int64_t stack_bytes(int64_t batch, int64_t m, int64_t n, int precision) {
+  return align256(batch * orth_chunks(m * n) * 8) + batch * matrix_bytes(m, n, splits(precision, m, n));
 }
 
-// one launch sequence over a.t.n stacks whose io fields x, out, mom, strides, m, n and g.batch are filled in
-static int orth_run(OrthArgs& a, OrthOut o, int steps, float ca, float cb, float cc, int precision, char* ws, hipStream_t st) {
-  int64_t sym = 0, full = 0, chunk = 0, split = 0, part = 0, off = 0;
+// one launch sequence over a.t.n stacks of one precision whose io fields x, out, mom, strides, m, n and g.batch are filled in
+template <class CS, class CF>
+static void launch_step(const OrthArgs& a, const OrthOut& o, int64_t sym, int64_t full, float ca, float cb, float cc, int flip, int last, hipStream_t st) {
+  orth_product_kernel<kGram, false, CS><<<dim3((unsigned)sym), dim3(CS::NT), 0, st>>>(a, o, ca, cb, cc, flip);
+  orth_product_kernel<kPoly, false, CS><<<dim3((unsigned)sym), dim3(CS::NT), 0, st>>>(a, o, ca, cb, cc, flip);
+  if (last) orth_product_kernel<kApply, true, CF><<<dim3((unsigned)full), dim3(CF::NT), 0, st>>>(a, o, ca, cb, cc, flip);
+  else orth_product_kernel<kApply, false, CF><<<dim3((unsigned)full), dim3(CF::NT), 0, st>>>(a, o, ca, cb, cc, flip);
+}
+
+static int64_t sym_tiles(const OrthArgs& a, int T) {
+  int64_t n = 0;
+  for (int s = 0; s < a.t.n; ++s) { const int64_t t = (a.t.g[s].rp + T - 1) / T; n += a.t.g[s].batch * (t * (t + 1) / 2); }
+  return n;
+}
+static int64_t full_tiles(const OrthArgs& a, int T) {
+  int64_t n = 0;
+  for (int s = 0; s < a.t.n; ++s) n += (int64_t)a.t.g[s].batch * ((a.t.g[s].rp + T - 1) / T) * ((a.t.g[s].cp + T - 1) / T);
+  return n;
+}
+
+static int orth_run(OrthArgs& a, OrthOut o, int steps, float ca, float cb, float cc, bool split, char* ws, hipStream_t st) {
+  int64_t chunk = 0, tiles = 0, part = 0, off = 0;
   for (int s = 0; s < a.t.n; ++s) part += (int64_t)a.t.g[s].batch * orth_chunks((int64_t)a.io[s].m * a.io[s].n);
   off = align256(part * 8);
   part = 0;
@@ -327,28 +562,51 @@ static int orth_run(OrthArgs& a, OrthOut o, int steps, float ca, float cb, float
     OrthIo& io = a.io[s];
     OrthGeom& g = a.t.g[s];
     g.r = io.m < io.n ? io.m : io.n; g.c = io.m < io.n ? io.n : io.m;
-    g.rp = (g.r + kTile - 1) / kTile * kTile; g.cp = (g.c + kTile - 1) / kTile * kTile;
-    g.split = precision == SNR_ORTH_FP32 || g.r <= 64;
-    const int64_t nti = g.rp / kTile, ntj = g.cp / kTile;
-    g.sym0 = (int)sym; g.full0 = (int)full; io.chunk0 = (int)chunk; io.split0 = (int)split;
+    g.rp = (g.r + kPad - 1) / kPad * kPad; g.cp = (g.c + kPad - 1) / kPad * kPad;
+    a.chunk0[s] = (int)chunk; a.split0[s] = (int)tiles;
     io.nchunk = orth_chunks((int64_t)io.m * io.n); io.part = part; g.ws = off;
-    sym += g.batch * (nti * (nti + 1) / 2); full += g.batch * nti * ntj; split += g.batch * nti * ntj;
+    tiles += (int64_t)g.batch * (g.rp / kPad) * (g.cp / kPad);
     chunk += (int64_t)g.batch * io.nchunk; part += (int64_t)g.batch * io.nchunk;
-    off += (int64_t)g.batch * orth_planes(g.rp, g.cp).total * 2;
-    if (sym > INT32_MAX || full > INT32_MAX || chunk > INT32_MAX) return SNR_ERR_SHAPE;
+    off += (int64_t)g.batch * orth_planes(g.rp, g.cp, split).total * 2;
+    if (tiles > INT32_MAX || chunk > INT32_MAX) return SNR_ERR_SHAPE;
   }
-  a.part = (double*)ws; a.ws = ws;
+  a.part = (double*)ws; a.ws = ws; a.split = split;
+  int ts = 64, tf = 64;
+  const int big = split ? 128 : 256;
+  const char* e1 = getenv("ORTH_TS"); const char* e2 = getenv("ORTH_TF");
+  while (tf < big && full_tiles(a, 2 * tf) >= 200) tf *= 2;
+  ts = tf;
+  if (e1) ts = atoi(e1); if (e2) tf = atoi(e2);
+  int64_t sym = 0, full = 0;
+  for (int s = 0; s < a.t.n; ++s) {
+    const OrthGeom& g = a.t.g[s];
+    a.sym0[s] = (int)sym; a.full0[s] = (int)full;
+    const int64_t t = (g.rp + ts - 1) / ts;
+    sym += g.batch * (t * (t + 1) / 2);
+    full += (int64_t)g.batch * ((g.rp + tf - 1) / tf) * ((g.cp + tf - 1) / tf);
+  }
   {
     ProfScope ps(K_ORTH_PREPARE, st);
     orth_reduce_kernel<<<dim3((unsigned)chunk), dim3(256), 0, st>>>(a);
-    orth_split_kernel<<<dim3((unsigned)split), dim3(256), 0, st>>>(a);
+    orth_split_kernel<<<dim3((unsigned)tiles), dim3(256), 0, st>>>(a);
   }
+  using S64 = TileCfg<64, 2, 2, true, NS64, 64>;
+  using S128 = TileCfg<128, 2, 2, true, 2, 64>;
+  using H64 = TileCfg<64, 2, 2, false, NH64, 64>;
+  using H128 = TileCfg<128, 2, 2, false, NH128, BK128>;
+  using H192 = TileCfg<192, 2, 2, false, 3, 64>;
+  using H256 = TileCfg<256, 2, 4, false, NH256, BK256>;
   for (int k = 0; k < steps; ++k) {
     const int flip = k & 1, last = k + 1 == steps;
     ProfScope ps(K_ORTH_PRODUCT, st);
-    orth_product_kernel<kGram><<<dim3((unsigned)sym), dim3(256), 0, st>>>(a, o, ca, cb, cc, flip, last);
-    orth_product_kernel<kPoly><<<dim3((unsigned)sym), dim3(256), 0, st>>>(a, o, ca, cb, cc, flip, last);
-    orth_product_kernel<kApply><<<dim3((unsigned)full), dim3(256), 0, st>>>(a, o, ca, cb, cc, flip, last);
+    const int key = (split ? 10000 : 0) + ts / 64 * 100 + tf / 64;
+#define SNR_STEP(k, A, B) case k: launch_step<A, B>(a, o, sym, full, ca, cb, cc, flip, last, st); break;
+    switch (key) {
+      SNR_STEP(101, H64, H64) SNR_STEP(202, H128, H128) SNR_STEP(303, H192, H192) SNR_STEP(304, H192, H256) SNR_STEP(404, H256, H256)
+      SNR_STEP(10101, S64, S64) SNR_STEP(10202, S128, S128)
+      default: return SNR_ERR_SHAPE;
+    }
+#undef SNR_STEP
   }
   return launch_status();
 }
@@ -356,7 +614,7 @@ static int orth_run(OrthArgs& a, OrthOut o, int steps, float ca, float cb, float
 extern "C" int64_t snr_orthogonalise_ws_bytes(int64_t batch, int64_t rows, int64_t cols, int precision) {
   if (precision != SNR_ORTH_FP16 && precision != SNR_ORTH_FP32) return SNR_ERR_UNSUPPORTED;
   const int st = stack_ok(batch, rows, cols);
-  return st != SNR_OK ? st : stack_bytes(batch, rows, cols);
+  return st != SNR_OK ? st : stack_bytes(batch, rows, cols, precision);
 }
 
 extern "C" int snr_orthogonalise(const void* x, int dtype, int64_t batch, int64_t rows, int64_t cols, int64_t x_batch_stride,
@@ -370,11 +628,11 @@ extern "C" int snr_orthogonalise(const void* x, int dtype, int64_t batch, int64_
   SNR_CHECK_ARG(orth_bounded(steps, a, b, c), SNR_ERR_UNSUPPORTED);
   OrthArgs A{};
   A.t.n = 1; A.t.g[0].batch = (int)batch;
-  A.io[0] = OrthIo{x, out, nullptr, x_batch_stride, x_row_stride, out_batch_stride, out_row_stride, (int)rows, (int)cols, 0, 0, 0, 0};
+  A.io[0] = OrthIo{x, out, nullptr, x_batch_stride, x_row_stride, out_batch_stride, out_row_stride, (int)rows, (int)cols, 0, 0};
   A.dtype = dtype; A.eps = eps;
   OrthOut o{};
   o.dtype = dtype;
-  return orth_run(A, o, steps, a, b, c, precision, (char*)ws, (hipStream_t)stream);
+  return orth_run(A, o, steps, a, b, c, splits(precision, rows, cols), (char*)ws, (hipStream_t)stream);
 }
 
 extern "C" int64_t snr_muon_ws_bytes(const snr_muon_item* items, int n_items, int precision) {
@@ -382,14 +640,17 @@ extern "C" int64_t snr_muon_ws_bytes(const snr_muon_item* items, int n_items, in
   if (n_items < 1) return SNR_ERR_SHAPE;
   if (precision != SNR_ORTH_FP16 && precision != SNR_ORTH_FP32) return SNR_ERR_UNSUPPORTED;
   int64_t most = 0;
-  for (int i = 0; i < n_items; i += kOrthMax) {      // one launch sequence after the other: they share the workspace
+  for (int pass = 0; pass < 2; ++pass) {      // as in snr_muon_step_multi
     int64_t sum = 0;
-    for (int k = i; k < n_items && k < i + kOrthMax; ++k) {
-      const int st = stack_ok(items[k].batch, items[k].rows, items[k].cols);
+    for (int i = 0, n = 0; i < n_items; ++i) {
+      const snr_muon_item& it = items[i];
+      const int st = stack_ok(it.batch, it.rows, it.cols);
       if (st != SNR_OK) return st;
-      sum += stack_bytes(items[k].batch, items[k].rows, items[k].cols);
+      if (splits(precision, it.rows, it.cols) != (pass == 0)) continue;
+      if (n == kOrthMax) { n = 0; sum = 0; }
+      sum += stack_bytes(it.batch, it.rows, it.cols, precision); ++n;
+      most = sum > most ? sum : most;
     }
-    most = sum > most ? sum : most;
   }
   return most;
 }
@@ -406,20 +667,25 @@ extern "C" int snr_muon_step_multi(const snr_muon_item* items, int n_items, floa
     SNR_CHECK_ARG(items[i].params && items[i].grads && items[i].momentum, SNR_ERR_NULL);
     SNR_CHECK_ARG(stack_ok(items[i].batch, items[i].rows, items[i].cols) == SNR_OK, SNR_ERR_SHAPE);
   }
-  for (int i = 0; i < n_items; i += kOrthMax) {
+  // stacks of one precision share a launch sequence; one sequence after the other, they share the workspace
+  for (int pass = 0; pass < 2; ++pass) {
     OrthArgs A{};
     OrthOut o{};
-    for (int k = i; k < n_items && k < i + kOrthMax; ++k) {
-      const snr_muon_item& it = items[k];
-      const int64_t mn = it.rows * it.cols;
-      A.t.g[k - i].batch = (int)it.batch;
-      A.io[k - i] = OrthIo{it.grads, it.params, it.momentum, mn, it.cols, mn, it.cols, (int)it.rows, (int)it.cols, 0, 0, 0, 0};
-      A.t.n = k - i + 1;
-    }
     A.mu = momentum; A.gscale = grad_scale; A.eps = eps; A.nesterov = nesterov;
     o.muon = 1; o.scale_mode = scale_mode; o.lr = lr; o.decay = weight_decay; o.st = state;
-    const int st = orth_run(A, o, steps, a, b, c, precision, (char*)ws, (hipStream_t)stream);
-    if (st != SNR_OK) return st;
+    for (int i = 0; i <= n_items; ++i) {
+      if (A.t.n == kOrthMax || (i == n_items && A.t.n)) {
+        const int st = orth_run(A, o, steps, a, b, c, pass == 0, (char*)ws, (hipStream_t)stream);
+        if (st != SNR_OK) return st;
+        A.t.n = 0;
+      }
+      if (i == n_items) break;
+      const snr_muon_item& it = items[i];
+      if (splits(precision, it.rows, it.cols) != (pass == 0)) continue;
+      const int64_t mn = it.rows * it.cols;
+      A.t.g[A.t.n].batch = (int)it.batch;
+      A.io[A.t.n++] = OrthIo{it.grads, it.params, it.momentum, mn, it.cols, mn, it.cols, (int)it.rows, (int)it.cols, 0, 0};
+    }
   }
   return SNR_OK;
 }
