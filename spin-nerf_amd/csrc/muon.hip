@@ -23,7 +23,7 @@ constexpr float kYs = 1024.f, kAs = 512.f;  // powers of two that the planes of 
 constexpr float kLo = 2048.f;               // ... and the lo planes on top
 
 struct OrthGeom {        // a stack of equal matrices
-  int r, c, rp, cp;      // sides of Y, and padded to the tile
+  int r, c, rp, cp;      // sides of Y, and padded
   int batch;
   int64_t ws;            // its planes
 };
@@ -74,6 +74,15 @@ __device__ __forceinline__ int find_stack(const int* first, int n, int block) {
   return __builtin_amdgcn_readfirstlane(__popcll(__ballot(mine)) - 1);
 }
 
+// a parameter p becomes keep p - lr_q x
+__device__ __forceinline__ void muon_rate(const OrthOut& o, const OrthIo& io, float& lr_q, float& keep) {
+  lr_q = 0.f; keep = 1.f;
+  if (!o.muon) return;
+  const float lr = o.st ? o.st->lr : o.lr, m = (float)io.m, n = (float)io.n;
+  const float q = o.scale_mode == SNR_MUON_SPECTRAL ? sqrtf(fmaxf(1.f, m / n)) : o.scale_mode == SNR_MUON_RMS ? 0.2f * sqrtf(fmaxf(m, n)) : 1.f;
+  lr_q = lr * q; keep = 1.f - lr * o.decay;
+}
+
 __device__ __forceinline__ float orth_load(const void* p, int64_t i, int dtype) {
   if (dtype == SNR_F32) return ((const float*)p)[i];
   if (dtype == SNR_F16) return (float)((const _Float16*)p)[i];
@@ -89,34 +98,78 @@ __device__ __forceinline__ void orth_split(float v, _Float16& hi, _Float16& lo) 
   lo = (_Float16)((v - (float)hi) * kLo);
 }
 
+// four consecutive elements; wide: they lie on their own size
+__device__ __forceinline__ f32x4 orth_load4(const void* p, int64_t i, int dtype, bool wide) {
+  typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+  typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+  if (wide) {
+    if (dtype == SNR_F32) return *(const f32x4*)((const float*)p + i);
+    if (dtype == SNR_F16) return __builtin_convertvector(*(const f16x4*)((const _Float16*)p + i), f32x4);
+    return __builtin_convertvector(*(const bf16x4*)((const __bf16*)p + i), f32x4);
+  }
+  f32x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = orth_load(p, i + e, dtype);
+  return v;
+}
+__device__ __forceinline__ bool on_grid(const void* p, int64_t a, int64_t b, int bytes) {   // address and strides are multiples of it
+  return (((uintptr_t)p | (uint64_t)a | (uint64_t)b) & (bytes - 1)) == 0;
+}
+__device__ __forceinline__ int type_bytes(int dtype) { return dtype == SNR_F32 ? 4 : 2; }
+
+// sum over the workgroup's 256 threads, in a fixed order; everyone gets it
+__device__ __forceinline__ double block_sum(double v) {
+  __shared__ double part[4];
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return (part[0] + part[1]) + (part[2] + part[3]);
+}
+
 // ---- 1. momentum (in place) and the partial sums of squares of the update, in 64 bits and in a fixed order ------------------
+// A pass over the input, bound by memory: 16 B a lane where its place allows.
 __global__ __launch_bounds__(256) void orth_reduce_kernel(OrthArgs a) {
   const int s = find_stack(a.chunk0, a.t.n, blockIdx.x);
   const OrthIo& io = a.io[s];
   const int k = blockIdx.x - a.chunk0[s], mat = k / io.nchunk, ch = k % io.nchunk;
   const int64_t count = (int64_t)io.m * io.n;
-  const int64_t per = (count + io.nchunk - 1) / io.nchunk, e0 = ch * per, e1 = e0 + per < count ? e0 + per : count;
   double sum = 0.0;
-  for (int64_t e = e0 + threadIdx.x; e < e1; e += 256) {
-    float u;
-    if (io.mom) {
-      const int64_t i = mat * count + e;
-      const float g = ((const float*)io.x)[i] * a.gscale, mo = io.mom[i] * a.mu + g;
-      io.mom[i] = mo;
-      u = a.nesterov ? g + a.mu * mo : mo;
-    } else {
-      u = orth_load(io.x, mat * io.xb + (e / io.n) * io.xr + e % io.n, a.dtype);
+  if (io.mom || io.xr == io.n) {                // elements one after the other
+    const int64_t per = ((count + io.nchunk - 1) / io.nchunk + 3) / 4 * 4, e0 = ch * per, e1 = e0 + per < count ? e0 + per : count;
+    const int64_t base = mat * io.xb;
+    const int b = io.mom ? 4 : type_bytes(a.dtype);
+    const bool wide = on_grid(io.x, base * b, 0, 4 * b) && (!io.mom || on_grid(io.mom, base * 4, 0, 16));
+    for (int64_t e = e0 + 4 * threadIdx.x; e < e1; e += 1024) {
+      f32x4 u = {0.f, 0.f, 0.f, 0.f};
+      const bool whole = e + 4 <= e1;
+      if (io.mom) {
+        float* M = io.mom + base + e;
+        f32x4 g = {0.f, 0.f, 0.f, 0.f}, mo = g;
+        if (whole) { g = orth_load4(io.x, base + e, SNR_F32, wide); mo = orth_load4(M, 0, SNR_F32, wide); }
+        else for (int i = 0; i < (int)(e1 - e); ++i) { g[i] = ((const float*)io.x)[base + e + i]; mo[i] = M[i]; }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { g[i] *= a.gscale; mo[i] = mo[i] * a.mu + g[i]; u[i] = a.nesterov ? g[i] + a.mu * mo[i] : mo[i]; }
+        if (whole && wide) *(f32x4*)M = mo;
+        else for (int i = 0; i < 4 && e + i < e1; ++i) M[i] = mo[i];
+      } else if (whole) {
+        u = orth_load4(io.x, base + e, a.dtype, wide);
+      } else {
+        for (int i = 0; i < (int)(e1 - e); ++i) u[i] = orth_load(io.x, base + e + i, a.dtype);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum += (double)u[i] * (double)u[i];
     }
-    sum += (double)u * (double)u;
+  } else {                                      // row by row
+    const int per = (io.m + io.nchunk - 1) / io.nchunk, r0 = ch * per, r1 = r0 + per < io.m ? r0 + per : io.m;
+    for (int r = r0; r < r1; ++r)
+      for (int c = threadIdx.x; c < io.n; c += 256) {
+        const float u = orth_load(io.x, mat * io.xb + r * io.xr + c, a.dtype);
+        sum += (double)u * (double)u;
+      }
   }
-  __shared__ double red[256];
-  red[threadIdx.x] = sum;
-  __syncthreads();
-  for (int w = 128; w > 0; w >>= 1) {
-    if ((int)threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) a.part[io.part + mat * io.nchunk + ch] = red[0];
+  sum = block_sum(sum);
+  if (threadIdx.x == 0) a.part[io.part + mat * io.nchunk + ch] = sum;
 }
 
 // ---- 2. Y = scaled input (transposed where it is tall) as planes, zero in the padding --------------------------------------------
@@ -128,43 +181,65 @@ __global__ __launch_bounds__(256) void orth_split_kernel(OrthArgs a) {
   const int k = blockIdx.x - a.split0[s], mat = k / (nti * ntj), t = k % (nti * ntj);
   const int i0 = t / ntj * kPad, j0 = t % ntj * kPad;
   const bool tall = io.m > io.n;
-  __shared__ double red[256];
   __shared__ float tile[kPad][kPad + 1];
   double sum = 0.0;
   for (int p = threadIdx.x; p < io.nchunk; p += 256) sum += a.part[io.part + mat * io.nchunk + p];
-  red[threadIdx.x] = sum;
-  __syncthreads();
-  for (int w = 128; w > 0; w >>= 1) {
-    if ((int)threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
-    __syncthreads();
-  }
-  const double norm = sqrt(red[0]);
+  const double norm = sqrt(block_sum(sum));
   const double scale = (double)kYs / (norm < (double)a.eps ? (double)a.eps : norm);   // (a NaN stays one)
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  // rows of the input are contiguous: lanes run along them
-  for (int q = w; q < kPad; q += 4) {
-    const int mi = tall ? j0 + q : i0 + q, nj = (tall ? i0 : j0) + lane;
-    float u = 0.f;
-    if (mi < io.m && nj < io.n) {
-      if (io.mom) {
-        const int64_t i = ((int64_t)mat * io.m + mi) * io.n + nj;
-        const float mo = io.mom[i];
-        u = a.nesterov ? ((const float*)io.x)[i] * a.gscale + a.mu * mo : mo;
-      } else {
-        u = orth_load(io.x, mat * io.xb + mi * io.xr + nj, a.dtype);
-      }
-      u = (float)((double)u * scale);
-    }
-    if (tall) tile[lane][q] = u; else tile[q][lane] = u;
-  }
-  __syncthreads();
   const OrthPlanes P = orth_planes(G.rp, G.cp, a.split);
   _Float16* W = (_Float16*)(a.ws + G.ws) + mat * P.total;
-  for (int q = w; q < kPad; q += 4) {
-    _Float16 hi, lo;
-    orth_split(tile[q][lane], hi, lo);
-    const int64_t y = (int64_t)(i0 + q) * G.cp + j0 + lane;
-    W[P.h[0] + y] = hi; W[P.l[0] + y] = lo;
+  typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+  // four columns a thread, sixteen rows of the input at once
+  const int b = io.mom ? 4 : type_bytes(a.dtype);
+  const bool wide = on_grid(io.x, mat * io.xb * b, io.xr * b, 4 * b) && (!io.mom || on_grid(io.mom, mat * io.xb * 4, io.xr * 4, 16));
+  const int c4 = 4 * (threadIdx.x & 15), r = threadIdx.x >> 4;
+#pragma unroll
+  for (int q = r; q < kPad; q += 16) {
+    const int mi = (tall ? j0 : i0) + q, nj = (tall ? i0 : j0) + c4;
+    f32x4 u = {0.f, 0.f, 0.f, 0.f};
+    if (mi < io.m && nj < io.n) {
+      const int64_t at = mat * io.xb + mi * io.xr + nj;
+      const bool whole = nj + 4 <= io.n;
+      if (io.mom) {
+        f32x4 mo = u;
+        if (whole) mo = orth_load4(io.mom, at, SNR_F32, wide);
+        else for (int e = 0; e < io.n - nj; ++e) mo[e] = io.mom[at + e];
+        u = mo;
+        if (a.nesterov) {
+          f32x4 g = {0.f, 0.f, 0.f, 0.f};
+          if (whole) g = orth_load4(io.x, at, SNR_F32, wide);
+          else for (int e = 0; e < io.n - nj; ++e) g[e] = ((const float*)io.x)[at + e];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) u[e] = g[e] * a.gscale + a.mu * mo[e];
+        }
+      } else if (whole) {
+        u = orth_load4(io.x, at, a.dtype, wide);
+      } else {
+        for (int e = 0; e < io.n - nj; ++e) u[e] = orth_load(io.x, at + e, a.dtype);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) u[e] = (float)((double)u[e] * scale);
+    }
+    if (tall) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) tile[c4 + e][q] = u[e];
+    } else {
+      f16x4 h, l;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { _Float16 x, y; orth_split(u[e], x, y); h[e] = x; l[e] = y; }
+      const int64_t y = (int64_t)(i0 + q) * G.cp + j0 + c4;
+      *(f16x4*)(W + P.h[0] + y) = h; *(f16x4*)(W + P.l[0] + y) = l;
+    }
+  }
+  if (!tall) return;
+  __syncthreads();
+#pragma unroll
+  for (int q = r; q < kPad; q += 16) {
+    f16x4 h, l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { _Float16 x, y; orth_split(tile[q][c4 + e], x, y); h[e] = x; l[e] = y; }
+    const int64_t y = (int64_t)(i0 + q) * G.cp + j0 + c4;
+    *(f16x4*)(W + P.h[0] + y) = h; *(f16x4*)(W + P.l[0] + y) = l;
   }
 }
 
@@ -299,6 +374,24 @@ template <bool LO> __device__ __forceinline__ void store16(const float (&v)[16],
   if constexpr (LO) { *(f16x8*)lo = l[0]; *(f16x8*)(lo + 8) = l[1]; }
 }
 
+__device__ __forceinline__ void store16_out(void* p, int64_t i, int dtype, const float (&v)[16]) {
+  typedef float f32v __attribute__((ext_vector_type(8)));
+#pragma unroll
+  for (int e = 0; e < 16; e += 8) {
+    f32v x;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) x[q] = v[e + q];
+    if (dtype == SNR_F32) {
+      *(f32x4*)((float*)p + i + e) = f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]};
+      *(f32x4*)((float*)p + i + e + 4) = f32x4{v[e + 4], v[e + 5], v[e + 6], v[e + 7]};
+    } else if (dtype == SNR_F16) {
+      *(f16x8*)((_Float16*)p + i + e) = __builtin_convertvector(x, f16x8);
+    } else {
+      *(bf16x8*)((__bf16*)p + i + e) = __builtin_convertvector(x, bf16x8);
+    }
+  }
+}
+
 // Workgroups go round the 8 XCDs, each with its own L2: number them so that an XCD has a run of neighbours, which share operand rows.
 __device__ __forceinline__ int xcd_block() {
   const int n = gridDim.x, q = n >> 3, rem = n & 7, x = blockIdx.x & 7;
@@ -320,13 +413,6 @@ template <int BAND> __device__ __forceinline__ void sym_tile(int t, int n, int& 
 
 template <int PHASE, bool last, class C>
 __global__ __launch_bounds__(C::NT) void orth_product_kernel(OrthArgs a, OrthOut o, float ca, float cb, float cc, int flip) {
-  // one array per stage: the compiler tells a DMA into one from a read of another by the object
-  __shared__ __attribute__((aligned(16))) char s0[C::STAGE > C::EPI ? C::STAGE : C::EPI];
-  __shared__ __attribute__((aligned(16))) char s1[C::STAGE];
-  __shared__ __attribute__((aligned(16))) char s2[C::STAGES > 2 ? C::STAGE : 16];
-  __shared__ __attribute__((aligned(16))) char s3[C::STAGES > 3 ? C::STAGE : 16];
-  char* const buf[4] = {s0, s1, s2, s3};
-  const unsigned at[4] = {lds_at(s0), lds_at(s1), lds_at(s2), lds_at(s3)};
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int block = xcd_block();
   const int s = find_stack(PHASE == kApply ? a.full0 : a.sym0, a.t.n, block);
@@ -345,6 +431,15 @@ __global__ __launch_bounds__(C::NT) void orth_product_kernel(OrthArgs a, OrthOut
   const OrthPlanes P = orth_planes(G.rp, G.cp, C::SPLIT);
   _Float16* W = (_Float16*)(a.ws + G.ws) + mat * P.total;
   const int64_t yh = flip ? P.h[1] : P.h[0], yl = flip ? P.l[1] : P.l[0];
+  const int wi = (wave / C::WJ) * (C::T / C::WI), wj = (wave % C::WJ) * (C::T / C::WJ);
+  f32x16 acc[C::TI][C::TJ] = {}, acl[C::SPLIT ? C::TI : 1][C::SPLIT ? C::TJ : 1] = {};
+  // one array per stage: no read of one is held up by a write to another
+  __shared__ __attribute__((aligned(16))) char s0[C::STAGE > C::EPI ? C::STAGE : C::EPI];
+  __shared__ __attribute__((aligned(16))) char s1[C::STAGE];
+  __shared__ __attribute__((aligned(16))) char s2[C::STAGES > 2 ? C::STAGE : 16];
+  __shared__ __attribute__((aligned(16))) char s3[C::STAGES > 3 ? C::STAGE : 16];
+  char* const buf[4] = {s0, s1, s2, s3};
+  const unsigned at[4] = {lds_at(s0), lds_at(s1), lds_at(s2), lds_at(s3)};
   const int K = PHASE == kGram ? G.cp : G.rp;
   const int64_t ldq = PHASE == kApply ? G.cp : 1;      // how far apart slices of Q lie, an element of k
   const int64_t ph = PHASE == kGram ? yh : PHASE == kPoly ? P.ah : P.bh, pl = PHASE == kGram ? yl : PHASE == kPoly ? P.al : P.bl;
@@ -364,8 +459,6 @@ __global__ __launch_bounds__(C::NT) void orth_product_kernel(OrthArgs a, OrthOut
       voff[1][q] = 2u * ((row < lq ? row : lq) * K + col);
     }
   }
-  const int wi = (wave / C::WJ) * (C::T / C::WI), wj = (wave % C::WJ) * (C::T / C::WJ);
-  f32x16 acc[C::TI][C::TJ] = {}, acl[C::SPLIT ? C::TI : 1][C::SPLIT ? C::TJ : 1] = {};
   const int n = K / C::BK;
   // Slice k's last 16 of K are multiplied behind the barrier that frees its buffer and shows slice k + 1, whose first fragments are
   // read under them; slice k + STAGES is fetched into the buffer at once.
@@ -407,13 +500,11 @@ __global__ __launch_bounds__(C::NT) void orth_product_kernel(OrthArgs a, OrthOut
   // 32 B a lane
   float (*blk)[36] = (float (*)[36])(s0 + wave * (32 * 36 * 4));
   float lr_q = 0.f, keep = 1.f;
-  if (PHASE == kApply && last && o.muon) {
-    const float lr = o.st ? o.st->lr : o.lr;
-    const float m = (float)a.io[s].m, n = (float)a.io[s].n;
-    const float q = o.scale_mode == SNR_MUON_SPECTRAL ? sqrtf(fmaxf(1.f, m / n)) : o.scale_mode == SNR_MUON_RMS ? 0.2f * sqrtf(fmaxf(m, n)) : 1.f;
-    lr_q = lr * q; keep = 1.f - lr * o.decay;
-  }
+  if (PHASE == kApply && last) muon_rate(o, a.io[s], lr_q, keep);
   const int row = lane >> 1, c0 = (lane & 1) * 16;
+  const OrthIo& io = a.io[s];
+  bool wide = false;                  // 16-byte pieces of the result
+  if (last) { const int b = o.muon ? 4 : type_bytes(o.dtype); wide = on_grid(io.out, mat * io.ob * b, io.orow * b, 16); }
 #pragma unroll
   for (int bi = 0; bi < C::TI; ++bi)
 #pragma unroll
@@ -457,20 +548,158 @@ __global__ __launch_bounds__(C::NT) void orth_product_kernel(OrthArgs a, OrthOut
         const int64_t yt = (int64_t)(j0 + row) * G.rp + i0 + c0;
         store16<C::SPLIT>(v, W + dh + yt, W + dl + yt);
       } else {
-        const OrthIo& io = a.io[s];
         const bool tall = io.m > io.n;
+        const int i = i0 + row, j = j0 + row;        // a row of the result: Y's or, where it is tall, Y's column
+        const int from = (tall ? i0 : j0) + c0, len = tall ? G.r : G.c;
+        const int64_t at = mat * io.ob + (tall ? j : i) * io.orow + from;
+        if (wide && (tall ? i0 : j0) + 32 <= len) {
+          const bool mine = (tall ? j : i) < (tall ? G.c : G.r);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int u = 2 * e + (lane >> 5), w = lane & 31;       // lanes along the result's rows
-          const int i = i0 + (tall ? w : u), j = j0 + (tall ? u : w);
-          if (i >= G.r || j >= G.c) continue;
-          const float x = (tall ? blk[w][u] : blk[u][w]) * (1.f / kYs);
-          const int64_t at = mat * io.ob + (tall ? (int64_t)j * io.orow + i : (int64_t)i * io.orow + j);
-          if (o.muon) { float* p = (float*)io.out + at; *p = *p * keep - lr_q * x; }
-          else orth_store(io.out, at, o.dtype, x);
+          for (int e = 0; e < 16; ++e) v[e] = (tall ? blk[c0 + e][row] : blk[row][c0 + e]) * (1.f / kYs);
+          if (!mine) {
+          } else if (o.muon) {
+            float* p = (float*)io.out + at;
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+              f32x4 x = *(const f32x4*)(p + e);
+#pragma unroll
+              for (int q = 0; q < 4; ++q) x[q] = x[q] * keep - lr_q * v[e + q];
+              *(f32x4*)(p + e) = x;
+            }
+          } else {
+            store16_out(io.out, at, o.dtype, v);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {             // lanes along the result's rows
+            const int u = 2 * e + (lane >> 5), w = lane & 31;
+            const int ei = i0 + (tall ? w : u), ej = j0 + (tall ? u : w);
+            if (ei >= G.r || ej >= G.c) continue;
+            const float x = (tall ? blk[w][u] : blk[u][w]) * (1.f / kYs);
+            const int64_t at1 = mat * io.ob + (tall ? (int64_t)ej * io.orow + ei : (int64_t)ei * io.orow + ej);
+            if (o.muon) { float* p = (float*)io.out + at1; *p = *p * keep - lr_q * x; }
+            else orth_store(io.out, at1, o.dtype, x);
+          }
         }
       }
     }
+}
+
+// ---- 4. small matrices: everything in one workgroup ----------------------------------------------------------------------------------
+// Where the shorter side is 64 or less and the longer one fits, a workgroup keeps a matrix from its input to its result: 17 launches
+// of a microsecond's work each become one.  Y stays in registers in 32 bits, as 32 x 32 blocks in the layout the matrix instructions
+// give them back in (NB a wave; a wave's block never moves); LDS holds the hi and lo planes that all four waves multiply from.  Always
+// the split products.  Bound by latency: four barriers and 3 (NB + 2) dependent rounds of LDS reads and products a step.
+constexpr int kSmallSide = 64, kSmallLong = 448;     // 448: Y's planes, A's and B's fill LDS
+template <int NB>
+__global__ __launch_bounds__(256) void orth_small_kernel(OrthArgs a, OrthOut o, float ca, float cb, float cc, int steps) {
+  constexpr int LD = 64 * NB + 8, LA = 64 + 8;       // rows in fp16: 16 B off a multiple of 128, so that 16 rows at one k spread over the banks
+  __shared__ __attribute__((aligned(16))) _Float16 yh[64 * LD], yl[64 * LD], ah[64 * LA], al[64 * LA], bh[64 * LA], bl[64 * LA];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int s = find_stack(a.sym0, a.t.n, blockIdx.x);
+  const OrthIo& io = a.io[s];
+  const int64_t mat = blockIdx.x - a.sym0[s];
+  const bool tall = io.m > io.n;
+  const int r = tall ? io.n : io.m, c = tall ? io.m : io.n;
+  const int lj = lane & 31, li = 4 * (lane >> 5);
+  float v[NB][16];
+  double sum = 0.0;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int i0 = 32 * ((wave + 4 * b) & 1) + li, j = 32 * ((wave + 4 * b) >> 1) + lj;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int i = i0 + 8 * (e >> 2) + (e & 3);
+      float u = 0.f;
+      if (i < r && j < c) {
+        const int64_t at = mat * io.xb + (tall ? j * io.xr + i : i * io.xr + j);
+        if (io.mom) {
+          const float g = ((const float*)io.x)[at] * a.gscale, mo = io.mom[at] * a.mu + g;
+          io.mom[at] = mo;
+          u = a.nesterov ? g + a.mu * mo : mo;
+        } else {
+          u = orth_load(io.x, at, a.dtype);
+        }
+      }
+      v[b][e] = u;
+      sum += (double)u * (double)u;
+    }
+  }
+  const double norm = sqrt(block_sum(sum));
+  const double scale = (double)kYs / (norm < (double)a.eps ? (double)a.eps : norm);   // (a NaN stays one)
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[b][e] = (float)((double)v[b][e] * scale);
+
+  // the operand fragments of one matrix instruction: 32 rows of a plane at 16 k, and 32 columns at 16 rows
+  auto rows = [&](const _Float16* p, int ld, int row, int k) { return *(const f16x8*)(p + (row + lj) * ld + 16 * k + 8 * (lane >> 5)); };
+  auto cols = [&](const _Float16* p, int ld, int k, int col) {
+    const _Float16* q = p + (16 * k + 8 * (lane >> 5) + ((lane & 15) >> 2)) * ld + col + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
+    union { s16x4 q[2]; f16x8 v; } u;
+    u.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)q);
+    u.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(q + 4 * ld));
+    return u.v;
+  };
+  auto mul = [&](f32x16& hi, f32x16& lo, f16x8 xh, f16x8 xl, f16x8 wh, f16x8 wl) {
+    hi = __builtin_amdgcn_mfma_f32_32x32x16_f16(xh, wh, hi, 0, 0, 0);
+    lo = __builtin_amdgcn_mfma_f32_32x32x16_f16(xh, wl, lo, 0, 0, 0);
+    lo = __builtin_amdgcn_mfma_f32_32x32x16_f16(xl, wh, lo, 0, 0, 0);
+  };
+  auto put = [&](_Float16* h, _Float16* l, int ld, int i0, int j, const float (&w)[16]) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int at = (i0 + 8 * (e >> 2) + (e & 3)) * ld + j;
+      orth_split(w[e], h[at], l[at]);
+    }
+  };
+  const int ai = 32 * (wave >> 1), aj = 32 * (wave & 1);     // this wave's block of A and B
+  for (int step = 0;; ++step) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) put(yh, yl, LD, 32 * ((wave + 4 * b) & 1) + li, 32 * ((wave + 4 * b) >> 1) + lj, v[b]);
+    __syncthreads();
+    f32x16 hi = {}, lo = {};
+#pragma unroll
+    for (int k = 0; k < 4 * NB; ++k) mul(hi, lo, rows(yh, LD, ai, k), rows(yl, LD, ai, k), rows(yh, LD, aj, k), rows(yl, LD, aj, k));
+    float w[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) w[e] = (hi[e] + lo[e] * (1.f / kLo)) * (kAs / (kYs * kYs));
+    put(ah, al, LA, ai + li, aj + lj, w);
+    __syncthreads();
+    hi = f32x16{}; lo = f32x16{};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) mul(hi, lo, rows(ah, LA, ai, k), rows(al, LA, ai, k), rows(ah, LA, aj, k), rows(al, LA, aj, k));
+#pragma unroll
+    for (int e = 0; e < 16; ++e) w[e] = cb * w[e] + cc * ((hi[e] + lo[e] * (1.f / kLo)) * (1.f / kAs));
+    put(bh, bl, LA, ai + li, aj + lj, w);
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const int i = 32 * ((wave + 4 * b) & 1), j = 32 * ((wave + 4 * b) >> 1);
+      hi = f32x16{}; lo = f32x16{};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) mul(hi, lo, rows(bh, LA, i, k), rows(bl, LA, i, k), cols(yh, LD, k, j), cols(yl, LD, k, j));
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[b][e] = ca * v[b][e] + (hi[e] + lo[e] * (1.f / kLo)) * (1.f / kAs);
+    }
+    if (step + 1 == steps) break;
+    __syncthreads();
+  }
+  float lr_q, keep;
+  muon_rate(o, io, lr_q, keep);
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int i0 = 32 * ((wave + 4 * b) & 1) + li, j = 32 * ((wave + 4 * b) >> 1) + lj;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int i = i0 + 8 * (e >> 2) + (e & 3);
+      if (i >= r || j >= c) continue;
+      const int64_t at = mat * io.ob + (tall ? j * io.orow + i : i * io.orow + j);
+      const float x = v[b][e] * (1.f / kYs);
+      if (o.muon) { float* p = (float*)io.out + at; *p = *p * keep - lr_q * x; }
+      else orth_store(io.out, at, o.dtype, x);
+    }
+  }
 }
 
 }  // namespace snr
@@ -506,107 +735,129 @@ static bool orth_bounded(int steps, double a, double b, double c) {
   return true;
 }
 
-#ifndef NS64
-#define NS64 4
-#define NH64 4
-#define NH128 2
-#define BK128 64
-#define NH256 2
-#define BK256 64
-#endif
 static int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
-static int orth_chunks(int64_t count) {
-  const int64_t n = (count + 4095) / 4096;
-  return (int)(n < 1 ? 1 : n > 1024 ? 1024 : n);
-}
-static int64_t matrix_bytes(int64_t m, int64_t n, bool split) {
-  const int64_t r = m < n ? m : n, c = m < n ? n : m;
-  return align256(orth_planes((int)((r + kPad - 1) / kPad * kPad), (int)((c + kPad - 1) / kPad * kPad), split).total * 2);
-}
 static const int64_t kMaxSide = 65536, kMaxBatch = 65536;
 static int stack_ok(int64_t batch, int64_t m, int64_t n) {
   if (batch < 1 || m < 1 || n < 1 || m > kMaxSide || n > kMaxSide || batch > kMaxBatch) return SNR_ERR_SHAPE;
   return SNR_OK;
 }
-static bool splits(int precision, int64_t m, int64_t n) { return precision == SNR_ORTH_FP32 || m <= 64 || n <= 64; }
-static int64_t stack_bytes(int64_t batch, int64_t m, int64_t n, int precision) {
-  return align256(batch * orth_chunks(m * n) * 8) + batch * matrix_bytes(m, n, splits(precision, m, n));
+// What a matrix goes through: the small kernel at NB = 1, 2, 4 or 7, the split products, or fp16 products.
+enum { kSmall1 = 0, kSmall2, kSmall4, kSmall7, kSplit, kHalf, kKinds };
+static int kind_of(int precision, int64_t m, int64_t n) {
+  const int64_t r = m < n ? m : n, c = m < n ? n : m;
+  if (r <= kSmallSide && c <= kSmallLong) return c <= 64 ? kSmall1 : c <= 128 ? kSmall2 : c <= 256 ? kSmall4 : kSmall7;
+  return precision == SNR_ORTH_FP32 || r <= 64 ? kSplit : kHalf;
 }
 
-// one launch sequence over a.t.n stacks of one precision whose io fields x, out, mom, strides, m, n and g.batch are filled in
-template <class CS, class CF>
-static void launch_step(const OrthArgs& a, const OrthOut& o, int64_t sym, int64_t full, float ca, float cb, float cc, int flip, int last, hipStream_t st) {
-  orth_product_kernel<kGram, false, CS><<<dim3((unsigned)sym), dim3(CS::NT), 0, st>>>(a, o, ca, cb, cc, flip);
-  orth_product_kernel<kPoly, false, CS><<<dim3((unsigned)sym), dim3(CS::NT), 0, st>>>(a, o, ca, cb, cc, flip);
-  if (last) orth_product_kernel<kApply, true, CF><<<dim3((unsigned)full), dim3(CF::NT), 0, st>>>(a, o, ca, cb, cc, flip);
-  else orth_product_kernel<kApply, false, CF><<<dim3((unsigned)full), dim3(CF::NT), 0, st>>>(a, o, ca, cb, cc, flip);
+using S64 = TileCfg<64, 2, 2, true, 2, 64>;
+using S128 = TileCfg<128, 2, 2, true, 2, 64>;
+using H64 = TileCfg<64, 2, 2, false, 3, 64>;
+using H128 = TileCfg<128, 2, 2, false, 2, 64>;
+using H192 = TileCfg<192, 2, 2, false, 3, 64>;
+using H256 = TileCfg<256, 2, 4, false, 2, 64>;
+template <int PHASE> struct Largest { using Cfg = H192; };
+template <> struct Largest<kApply> { using Cfg = H256; };
+
+// Everything of a launch sequence that follows from its stacks' sizes; also the bytes of its workspace.
+struct OrthPlan { int ts, tf; int64_t sym, full, chunk, split, bytes; };
+
+static int64_t sym_tiles(const OrthGeom& g, int T) { const int64_t t = (g.rp + T - 1) / T; return g.batch * (t * (t + 1) / 2); }
+static int64_t full_tiles(const OrthGeom& g, int T) { return (int64_t)g.batch * ((g.rp + T - 1) / T) * ((g.cp + T - 1) / T); }
+
+// The largest tile that still makes work for most of the chip: a larger one reads less per product, but a workgroup has a compute
+// unit to itself (128: two share one) and idle ones are worth more.  Us a product at 64 / 128 / 192 / 256, fp16: symmetric, 4096^2:
+// 132 / 113 / 95 / 120, 2048^2: 25 / 27 / 40 / 60; B Y, 4096^2: 249 / 170 / 198 / 135, 2048 x 8192: 125 / 89 / 102 / 80, 4 x 1024^2 and
+// 2 of 1024 x 4096: 55 / 47 / 62 / 55.  fp32 (no larger tile fits LDS twice), 2048^2: 53 / 54, 67 / 65; 14 x 256^2: 7 / 13.
+template <class F> static int pick_tile(const OrthArgs& a, bool split, int largest, F tiles) {
+  int64_t n[2] = {0, 0};
+  for (int s = 0; s < a.t.n; ++s) { n[0] += tiles(a.t.g[s], largest); n[1] += tiles(a.t.g[s], 128); }
+  const int cus = cu_count();
+  if (!split && n[0] >= cus * 3 / 4) return largest;
+  return n[1] >= cus / 2 ? 128 : 64;
 }
 
-static int64_t sym_tiles(const OrthArgs& a, int T) {
-  int64_t n = 0;
-  for (int s = 0; s < a.t.n; ++s) { const int64_t t = (a.t.g[s].rp + T - 1) / T; n += a.t.g[s].batch * (t * (t + 1) / 2); }
-  return n;
-}
-static int64_t full_tiles(const OrthArgs& a, int T) {
-  int64_t n = 0;
-  for (int s = 0; s < a.t.n; ++s) n += (int64_t)a.t.g[s].batch * ((a.t.g[s].rp + T - 1) / T) * ((a.t.g[s].cp + T - 1) / T);
-  return n;
-}
-
-static int orth_run(OrthArgs& a, OrthOut o, int steps, float ca, float cb, float cc, bool split, char* ws, hipStream_t st) {
-  int64_t chunk = 0, tiles = 0, part = 0, off = 0;
-  for (int s = 0; s < a.t.n; ++s) part += (int64_t)a.t.g[s].batch * orth_chunks((int64_t)a.io[s].m * a.io[s].n);
-  off = align256(part * 8);
-  part = 0;
+static int orth_plan(OrthArgs& a, int kind, OrthPlan& p) {
+  int64_t off = 0, part = 0;
+  const bool split = kind != kHalf;
+  p.chunk = p.split = p.sym = p.full = 0;
+  if (kind < kSplit) {                       // a workgroup a matrix, no workspace
+    for (int s = 0; s < a.t.n; ++s) { a.sym0[s] = (int)p.sym; p.sym += a.t.g[s].batch; }
+    p.bytes = 256;
+    return SNR_OK;
+  }
   for (int s = 0; s < a.t.n; ++s) {
     OrthIo& io = a.io[s];
     OrthGeom& g = a.t.g[s];
     g.r = io.m < io.n ? io.m : io.n; g.c = io.m < io.n ? io.n : io.m;
     g.rp = (g.r + kPad - 1) / kPad * kPad; g.cp = (g.c + kPad - 1) / kPad * kPad;
-    a.chunk0[s] = (int)chunk; a.split0[s] = (int)tiles;
-    io.nchunk = orth_chunks((int64_t)io.m * io.n); io.part = part; g.ws = off;
-    tiles += (int64_t)g.batch * (g.rp / kPad) * (g.cp / kPad);
-    chunk += (int64_t)g.batch * io.nchunk; part += (int64_t)g.batch * io.nchunk;
-    off += (int64_t)g.batch * orth_planes(g.rp, g.cp, split).total * 2;
-    if (tiles > INT32_MAX || chunk > INT32_MAX) return SNR_ERR_SHAPE;
+    const int64_t n = ((int64_t)io.m * io.n + 8191) / 8192;
+    io.nchunk = (int)(n > 1024 ? 1024 : n);
+    io.part = part; part += (int64_t)g.batch * io.nchunk;
+    a.chunk0[s] = (int)p.chunk; p.chunk += (int64_t)g.batch * io.nchunk;
+    a.split0[s] = (int)p.split; p.split += (int64_t)g.batch * (g.rp / kPad) * (g.cp / kPad);
+    g.ws = off; off += (int64_t)g.batch * orth_planes(g.rp, g.cp, split).total * 2;
+    if (p.chunk > INT32_MAX || p.split > INT32_MAX) return SNR_ERR_SHAPE;
   }
-  a.part = (double*)ws; a.ws = ws; a.split = split;
-  int ts = 64, tf = 64;
-  const int big = split ? 128 : 256;
-  const char* e1 = getenv("ORTH_TS"); const char* e2 = getenv("ORTH_TF");
-  while (tf < big && full_tiles(a, 2 * tf) >= 200) tf *= 2;
-  ts = tf;
-  if (e1) ts = atoi(e1); if (e2) tf = atoi(e2);
-  int64_t sym = 0, full = 0;
-  for (int s = 0; s < a.t.n; ++s) {
-    const OrthGeom& g = a.t.g[s];
-    a.sym0[s] = (int)sym; a.full0[s] = (int)full;
-    const int64_t t = (g.rp + ts - 1) / ts;
-    sym += g.batch * (t * (t + 1) / 2);
-    full += (int64_t)g.batch * ((g.rp + tf - 1) / tf) * ((g.cp + tf - 1) / tf);
+  p.ts = pick_tile(a, split, 192, sym_tiles);
+  p.tf = pick_tile(a, split, 256, full_tiles);
+  for (int s = 0; s < a.t.n; ++s) {          // (no more than the split's: a tile holds 64 x 64 or more)
+    a.sym0[s] = (int)p.sym; a.full0[s] = (int)p.full;
+    p.sym += sym_tiles(a.t.g[s], p.ts); p.full += full_tiles(a.t.g[s], p.tf);
+  }
+  const int64_t at_part = align256(off);     // the planes come first: on 256 bytes
+  p.bytes = at_part + align256(part * 8);
+  a.part = (double*)(a.ws + at_part);
+  a.split = split;
+  return SNR_OK;
+}
+
+template <int PHASE, bool last, class C>
+static void launch(const OrthArgs& a, const OrthOut& o, int64_t n, float ca, float cb, float cc, int flip, hipStream_t st) {
+  orth_product_kernel<PHASE, last, C><<<dim3((unsigned)n), dim3(C::NT), 0, st>>>(a, o, ca, cb, cc, flip);
+}
+template <int PHASE, bool last>
+static void launch_tile(bool split, int T, const OrthArgs& a, const OrthOut& o, int64_t n, float ca, float cb, float cc, int flip, hipStream_t st) {
+  if (split) {
+    if (T == 64) launch<PHASE, last, S64>(a, o, n, ca, cb, cc, flip, st);
+    else launch<PHASE, last, S128>(a, o, n, ca, cb, cc, flip, st);
+  } else if (T == 64) {
+    launch<PHASE, last, H64>(a, o, n, ca, cb, cc, flip, st);
+  } else if (T == 128) {
+    launch<PHASE, last, H128>(a, o, n, ca, cb, cc, flip, st);
+  } else {
+    launch<PHASE, last, typename Largest<PHASE>::Cfg>(a, o, n, ca, cb, cc, flip, st);
+  }
+}
+
+// one launch sequence over a.t.n stacks of one precision whose io fields x, out, mom, strides, m, n and g.batch are filled in
+static int orth_run(OrthArgs& a, const OrthOut& o, int steps, float ca, float cb, float cc, int kind, char* ws, hipStream_t st) {
+  a.ws = ws;
+  OrthPlan p;
+  const int ok = orth_plan(a, kind, p);
+  if (ok != SNR_OK) return ok;
+  const bool split = kind != kHalf;
+  if (kind < kSplit) {
+    ProfScope ps(K_ORTH_SMALL, st);
+    const dim3 n((unsigned)p.sym), t(256);
+    switch (kind) {
+      case kSmall1: orth_small_kernel<1><<<n, t, 0, st>>>(a, o, ca, cb, cc, steps); break;
+      case kSmall2: orth_small_kernel<2><<<n, t, 0, st>>>(a, o, ca, cb, cc, steps); break;
+      case kSmall4: orth_small_kernel<4><<<n, t, 0, st>>>(a, o, ca, cb, cc, steps); break;
+      default: orth_small_kernel<7><<<n, t, 0, st>>>(a, o, ca, cb, cc, steps);
+    }
+    return launch_status();
   }
   {
     ProfScope ps(K_ORTH_PREPARE, st);
-    orth_reduce_kernel<<<dim3((unsigned)chunk), dim3(256), 0, st>>>(a);
-    orth_split_kernel<<<dim3((unsigned)tiles), dim3(256), 0, st>>>(a);
+    orth_reduce_kernel<<<dim3((unsigned)p.chunk), dim3(256), 0, st>>>(a);
+    orth_split_kernel<<<dim3((unsigned)p.split), dim3(256), 0, st>>>(a);
   }
-  using S64 = TileCfg<64, 2, 2, true, NS64, 64>;
-  using S128 = TileCfg<128, 2, 2, true, 2, 64>;
-  using H64 = TileCfg<64, 2, 2, false, NH64, 64>;
-  using H128 = TileCfg<128, 2, 2, false, NH128, BK128>;
-  using H192 = TileCfg<192, 2, 2, false, 3, 64>;
-  using H256 = TileCfg<256, 2, 4, false, NH256, BK256>;
   for (int k = 0; k < steps; ++k) {
-    const int flip = k & 1, last = k + 1 == steps;
     ProfScope ps(K_ORTH_PRODUCT, st);
-    const int key = (split ? 10000 : 0) + ts / 64 * 100 + tf / 64;
-#define SNR_STEP(k, A, B) case k: launch_step<A, B>(a, o, sym, full, ca, cb, cc, flip, last, st); break;
-    switch (key) {
-      SNR_STEP(101, H64, H64) SNR_STEP(202, H128, H128) SNR_STEP(303, H192, H192) SNR_STEP(304, H192, H256) SNR_STEP(404, H256, H256)
-      SNR_STEP(10101, S64, S64) SNR_STEP(10202, S128, S128)
-      default: return SNR_ERR_SHAPE;
-    }
-#undef SNR_STEP
+    launch_tile<kGram, false>(split, p.ts, a, o, p.sym, ca, cb, cc, k & 1, st);
+    launch_tile<kPoly, false>(split, p.ts, a, o, p.sym, ca, cb, cc, k & 1, st);
+    if (k + 1 == steps) launch_tile<kApply, true>(split, p.tf, a, o, p.full, ca, cb, cc, k & 1, st);
+    else launch_tile<kApply, false>(split, p.tf, a, o, p.full, ca, cb, cc, k & 1, st);
   }
   return launch_status();
 }
@@ -614,7 +865,12 @@ static int orth_run(OrthArgs& a, OrthOut o, int steps, float ca, float cb, float
 extern "C" int64_t snr_orthogonalise_ws_bytes(int64_t batch, int64_t rows, int64_t cols, int precision) {
   if (precision != SNR_ORTH_FP16 && precision != SNR_ORTH_FP32) return SNR_ERR_UNSUPPORTED;
   const int st = stack_ok(batch, rows, cols);
-  return st != SNR_OK ? st : stack_bytes(batch, rows, cols, precision);
+  if (st != SNR_OK) return st;
+  OrthArgs A{};
+  OrthPlan p;
+  A.t.n = 1; A.t.g[0].batch = (int)batch; A.io[0].m = (int)rows; A.io[0].n = (int)cols;
+  const int ok = orth_plan(A, kind_of(precision, rows, cols), p);
+  return ok != SNR_OK ? ok : p.bytes;
 }
 
 extern "C" int snr_orthogonalise(const void* x, int dtype, int64_t batch, int64_t rows, int64_t cols, int64_t x_batch_stride,
@@ -632,27 +888,47 @@ extern "C" int snr_orthogonalise(const void* x, int dtype, int64_t batch, int64_
   A.dtype = dtype; A.eps = eps;
   OrthOut o{};
   o.dtype = dtype;
-  return orth_run(A, o, steps, a, b, c, splits(precision, rows, cols), (char*)ws, (hipStream_t)stream);
+  return orth_run(A, o, steps, a, b, c, kind_of(precision, rows, cols), (char*)ws, (hipStream_t)stream);
+}
+
+// The launch sequences of a list of items: stacks of one kind share one, kOrthMax at a time; they run one after the other and share
+// the workspace.  F(OrthArgs&, kind) returns a status.
+template <class F> static int for_sequences(const snr_muon_item* items, int n_items, int precision, F f) {
+  for (int kind = 0; kind < kKinds; ++kind) {
+    OrthArgs A{};
+    for (int i = 0; i <= n_items; ++i) {
+      if (A.t.n == kOrthMax || (i == n_items && A.t.n)) {
+        const int st = f(A, kind);
+        if (st != SNR_OK) return st;
+        A.t.n = 0;
+      }
+      if (i == n_items) break;
+      const snr_muon_item& it = items[i];
+      if (kind_of(precision, it.rows, it.cols) != kind) continue;
+      const int64_t mn = it.rows * it.cols;
+      A.t.g[A.t.n].batch = (int)it.batch;
+      A.io[A.t.n++] = OrthIo{it.grads, it.params, it.momentum, mn, it.cols, mn, it.cols, (int)it.rows, (int)it.cols, 0, 0};
+    }
+  }
+  return SNR_OK;
 }
 
 extern "C" int64_t snr_muon_ws_bytes(const snr_muon_item* items, int n_items, int precision) {
   if (!items) return SNR_ERR_NULL;
   if (n_items < 1) return SNR_ERR_SHAPE;
   if (precision != SNR_ORTH_FP16 && precision != SNR_ORTH_FP32) return SNR_ERR_UNSUPPORTED;
-  int64_t most = 0;
-  for (int pass = 0; pass < 2; ++pass) {      // as in snr_muon_step_multi
-    int64_t sum = 0;
-    for (int i = 0, n = 0; i < n_items; ++i) {
-      const snr_muon_item& it = items[i];
-      const int st = stack_ok(it.batch, it.rows, it.cols);
-      if (st != SNR_OK) return st;
-      if (splits(precision, it.rows, it.cols) != (pass == 0)) continue;
-      if (n == kOrthMax) { n = 0; sum = 0; }
-      sum += stack_bytes(it.batch, it.rows, it.cols, precision); ++n;
-      most = sum > most ? sum : most;
-    }
+  for (int i = 0; i < n_items; ++i) {
+    const int st = stack_ok(items[i].batch, items[i].rows, items[i].cols);
+    if (st != SNR_OK) return st;
   }
-  return most;
+  int64_t most = 0;
+  const int st = for_sequences(items, n_items, precision, [&](OrthArgs& A, int kind) {
+    OrthPlan p;
+    const int ok = orth_plan(A, kind, p);
+    most = ok == SNR_OK && p.bytes > most ? p.bytes : most;
+    return ok;
+  });
+  return st != SNR_OK ? st : most;
 }
 
 extern "C" int snr_muon_step_multi(const snr_muon_item* items, int n_items, float lr, float momentum, int nesterov, float weight_decay,
@@ -667,25 +943,10 @@ extern "C" int snr_muon_step_multi(const snr_muon_item* items, int n_items, floa
     SNR_CHECK_ARG(items[i].params && items[i].grads && items[i].momentum, SNR_ERR_NULL);
     SNR_CHECK_ARG(stack_ok(items[i].batch, items[i].rows, items[i].cols) == SNR_OK, SNR_ERR_SHAPE);
   }
-  // stacks of one precision share a launch sequence; one sequence after the other, they share the workspace
-  for (int pass = 0; pass < 2; ++pass) {
-    OrthArgs A{};
-    OrthOut o{};
+  OrthOut o{};
+  o.muon = 1; o.scale_mode = scale_mode; o.lr = lr; o.decay = weight_decay; o.st = state;
+  return for_sequences(items, n_items, precision, [&](OrthArgs& A, int kind) {
     A.mu = momentum; A.gscale = grad_scale; A.eps = eps; A.nesterov = nesterov;
-    o.muon = 1; o.scale_mode = scale_mode; o.lr = lr; o.decay = weight_decay; o.st = state;
-    for (int i = 0; i <= n_items; ++i) {
-      if (A.t.n == kOrthMax || (i == n_items && A.t.n)) {
-        const int st = orth_run(A, o, steps, a, b, c, pass == 0, (char*)ws, (hipStream_t)stream);
-        if (st != SNR_OK) return st;
-        A.t.n = 0;
-      }
-      if (i == n_items) break;
-      const snr_muon_item& it = items[i];
-      if (splits(precision, it.rows, it.cols) != (pass == 0)) continue;
-      const int64_t mn = it.rows * it.cols;
-      A.t.g[A.t.n].batch = (int)it.batch;
-      A.io[A.t.n++] = OrthIo{it.grads, it.params, it.momentum, mn, it.cols, mn, it.cols, (int)it.rows, (int)it.cols, 0, 0};
-    }
-  }
-  return SNR_OK;
+    return orth_run(A, o, steps, a, b, c, kind, (char*)ws, (hipStream_t)stream);
+  });
 }

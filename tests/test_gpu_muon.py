@@ -70,7 +70,7 @@ def check(got, x, precision, steps=5, coefficients=NS, eps=1e-7):
     assert bool((off <= tol).all()), (float((off / size.clamp(min=1e-30)).max()), float((tol / size.clamp(min=1e-30)).max()))
 
 
-SHAPES = [(1, 1), (1, 7), (5, 1), (2, 3), (31, 33), (64, 64), (63, 65), (65, 64), (16, 200), (200, 16), (128, 283), (256, 256), (256, 319),
+SHAPES = [(1, 1), (64, 448), (449, 64), (33, 129), (257, 60), (1, 7), (5, 1), (2, 3), (31, 33), (64, 64), (63, 65), (65, 64), (16, 200), (200, 16), (128, 283), (256, 256), (256, 319),
           (319, 256), (130, 129), (1000, 333), (40, 1500)]
 
 
@@ -262,7 +262,10 @@ def test_muon_leaves_the_surroundings_alone(S):
     flat = torch.full((3 * 4000,), 7.0, device="cuda")
     p, g, m = flat[13:13 + 50 * 61].view(50, 61), torch.randn(50, 61, device="cuda"), torch.zeros(50, 61, device="cuda")
     S.muon_step_([p], [g], [m], 0.02)
-    assert bool((flat[:13] == 7).all()) and bool((flat[13 + 50 * 61:] == 7).all()) and not bool((p == 7).any())
+    assert bool((flat[:13] == 7).all()) and bool((flat[13 + 50 * 61:] == 7).all())
+    # an entry of 7 stays where its step is below half an ulp, 2.4e-7: |O| < 1.2e-5 where O has a deviation of 61 ** -0.5 = 0.13,
+    # one entry in 13 000 of these 3050
+    assert float((p == 7).float().mean()) < 0.01
 
 
 def test_set_captured_into_a_graph_and_replayed(S):

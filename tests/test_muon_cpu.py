@@ -73,7 +73,8 @@ def test_entry_points_refuse_before_any_device_access(S):
 def test_workspace_sizes(S):
     lib, L = S._lib.load(), S._lib
     one = lib.snr_orthogonalise_ws_bytes(1, 256, 256, 0)
-    assert one >= 8 * 256 * 256 * 2 and lib.snr_orthogonalise_ws_bytes(4, 256, 256, 0) >= 4 * 8 * 256 * 256 * 2
+    least = 3 * 256 * 256 * 2      # X in 22 bits and the Gram matrix
+    assert one >= least and lib.snr_orthogonalise_ws_bytes(4, 256, 256, 0) >= 4 * least
     assert lib.snr_orthogonalise_ws_bytes(1, 256, 319, 1) == lib.snr_orthogonalise_ws_bytes(1, 319, 256, 1) > one
     assert lib.snr_orthogonalise_ws_bytes(0, 8, 8, 0) == -2 and lib.snr_orthogonalise_ws_bytes(1, 8, 8, 5) == -3
     assert lib.snr_orthogonalise_ws_bytes(1, 65536, 65536, 1) > 1 << 34          # sizes are 64-bit
