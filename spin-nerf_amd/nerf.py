@@ -100,6 +100,27 @@ class NeRF(nn.Module):
         return OrderedDict((k, v) for k, v in self.named_views(flat).items()
                            if k.rsplit(".", 1)[0] not in self._UNREGISTERED)
 
+    def hidden_matrices(self):
+        """names of the hidden weight matrices, the ones an orthogonalised update is meant for: both sides are features of the
+        network.  Not among them: the input layer, the heads, and views_linears.0 of a network without view directions (never used)"""
+        names = [f"pts_linears.{i}" for i in range(1, self.D)]
+        return [n + ".weight" for n in names + (["views_linears.0", "feature_linear"] if self.use_viewdirs else [])]
+
+    def split_hidden(self, flat=None):
+        """(hidden matrices, the ranges between them) as views of a flat buffer; together they cover it"""
+        flat = self.flat if flat is None else flat
+        hidden, mats, rest, o, o0 = set(self.hidden_matrices()), [], [], 0, 0
+        for k, v in self.named_views(flat).items():
+            if k in hidden:
+                mats.append(v)
+                if o > o0:
+                    rest.append(flat[o0:o])
+                o0 = o + v.numel()
+            o += v.numel()
+        if o > o0:
+            rest.append(flat[o0:o])
+        return mats, rest
+
     def _linear(self, name):
         v = self.named_views(self.flat.detach())
         return _LinearView(v[name + ".weight"], v[name + ".bias"])

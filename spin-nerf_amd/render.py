@@ -341,13 +341,14 @@ def _load_per_layer_adam(optimizer, osd, nets):
         optimizer.state[n.flat] = {'step': torch.tensor(float(stp)), 'exp_avg': m, 'exp_avg_sq': v}
 
 
-def scatter_per_layer_adam(st, nets, moments):
+def scatter_per_layer_adam(st, nets, moments, muon=False):
     """Per-layer torch.optim.Adam state `st` (index -> {step, exp_avg, exp_avg_sq}, coarse network first) into the flat
     moment buffers `moments` = [(m, v)] of `nets`; returns the step count of each network.  A layer without an entry is
     accepted where the reference gives that layer no gradient — views_linears.* of a network built without
     use_viewdirs is registered but never used (helpers:86-90, 118-120), so torch.optim.Adam creates no state for it and
     the indices of a genuine reference checkpoint have holes there: its moments stay zero.  Anything else that does not
-    correspond raises (a resumed run must not silently restart moments, bias correction and learning-rate decay)."""
+    correspond raises (a resumed run must not silently restart moments, bias correction and learning-rate decay).
+    ``muon``: the hidden matrices' entries hold a momentum_buffer in place of Adam's moments (RenderTrainer(muon=...)); it goes to m."""
     n_params = sum(len(n.param_views()) for n in nets)
     unknown = [k for k in st if not (isinstance(k, int) and 0 <= k < n_params)]
     if unknown:
@@ -363,6 +364,16 @@ def scatter_per_layer_adam(st, nets, moments):
             if e is None:
                 if not (name.startswith("views_linears") and not getattr(n, "use_viewdirs", True)):
                     raise RuntimeError(f"optimizer_state_dict has no Adam state for parameter {idx} ({name}): cannot resume the optimizer")
+            elif ('momentum_buffer' in e) != (muon and name in n.hidden_matrices()):
+                raise RuntimeError(f"optimizer state of parameter {idx} ({name}): " + (
+                    "a momentum buffer, written by RenderTrainer(muon=...): resume with RenderTrainer(muon=...).load_checkpoint"
+                    if 'momentum_buffer' in e else "Adam moments where RenderTrainer(muon=...) keeps a momentum buffer: load the networks' "
+                    "weights alone and start the optimizer anew"))
+            elif 'momentum_buffer' in e:
+                if e['momentum_buffer'].numel() != mv.numel():
+                    raise RuntimeError(f"momentum of parameter {idx} ({name}) has {e['momentum_buffer'].numel()} elements, the layer {mv.numel()}")
+                mv.copy_(e['momentum_buffer'].reshape(mv.shape))
+                steps.add(float(e['step']))
             else:
                 if e['exp_avg'].numel() != mv.numel():
                     raise RuntimeError(f"Adam state of parameter {idx} ({name}) has {e['exp_avg'].numel()} elements, the layer {mv.numel()}")

@@ -27,8 +27,12 @@ def img2mse(x, y):
 
 class RenderTrainer:
     def __init__(self, render_kwargs_train, lrate=5e-4, lrate_decay=250, world_size=1, process_group=None,
-                 optimizer=None, start=None, graph=False):
-        """``optimizer`` / ``start`` = what create_nerf() returned: when it reloaded a checkpoint (run_nerf.py:448-462)
+                 optimizer=None, start=None, graph=False, muon=None):
+        """``muon``: None = Adam on every parameter, like the reference; True or a dict of muon_step_'s settings (momentum, nesterov,
+        weight_decay, scale, steps, coefficients, eps, precision) = orthogonalised updates for the networks' hidden matrices
+        (NeRF.hidden_matrices) and Adam for the rest, at one learning rate: scale defaults to "rms", whose steps are about Adam's size.
+
+        ``optimizer`` / ``start`` = what create_nerf() returned: when it reloaded a checkpoint (run_nerf.py:448-462)
         the Adam moments, the step count and the learning rate it restored continue here (a resumed run must not
         restart the bias correction and the lr decay); an optimizer whose state does not cover every network raises."""
         self.kw = dict(render_kwargs_train)
@@ -43,6 +47,17 @@ class RenderTrainer:
         self._lr = lrate              # rate the NEXT step uses (run_nerf.py:1616-1622 sets it after each step)
         self.m = [torch.zeros_like(n.flat.data) for n in self.nets]
         self.v = [torch.zeros_like(n.flat.data) for n in self.nets]
+        self.muon = None              # else: the hidden matrices' parts of self.m are momentum buffers, those of self.v stay zero
+        if muon:
+            self.muon = dict(momentum=0.95, nesterov=True, weight_decay=0.0, scale="rms", steps=5, coefficients=ops.NEWTON_SCHULZ,
+                             eps=1e-7, precision="fp32")
+            unknown = set(muon) - set(self.muon) if isinstance(muon, dict) else set()
+            if unknown:
+                raise ValueError(f"RenderTrainer: muon has no settings {sorted(unknown)}; there are {sorted(self.muon)}")
+            self.muon.update(muon if isinstance(muon, dict) else {})
+            bad = [type(n).__name__ for n in self.nets if not hasattr(n, "split_hidden")]
+            if bad:
+                raise NotImplementedError(f"RenderTrainer: muon is for NeRF networks, whose hidden layers are matrices of their own; got {bad}")
         # in-kernel random draws (Philox key / running call counter); ranks draw different streams
         self._seed = (torch.initial_seed() + 0x9E3779B97F4A7C15 * (self._rank() + 1)) & 0xFFFFFFFFFFFFFFFF
         self._draws = 0
@@ -74,6 +89,9 @@ class RenderTrainer:
         """continue from a torch.optim.Adam over the networks' flat parameters (create_nerf's return value)"""
         st = optimizer.state
         have = [n.flat in st and 'exp_avg' in st[n.flat] for n in self.nets]
+        if any(have) and self.muon is not None:
+            raise RuntimeError("the optimizer holds Adam state for the hidden matrices; RenderTrainer(muon=...) resumes its own checkpoints "
+                               "(load_checkpoint) or starts anew")
         if any(have) and not all(have):
             raise RuntimeError("the optimizer holds Adam state for some of the networks only; cannot resume")
         if all(have) and self.nets:
@@ -317,9 +335,11 @@ class RenderTrainer:
             grads = {id(net_c): g_c}
             if two:
                 grads[id(net_f)] = g_f
+            if self.muon is not None:
+                self._muon_step([(n, grads[id(n)], m, v) for n, m, v in zip(self.nets, self.m, self.v) if id(n) in grads], state=G["state"])
             for n, m, v in zip(self.nets, self.m, self.v):
                 gr = grads.get(id(n))
-                if gr is None:
+                if gr is None or self.muon is not None:
                     continue
                 check(lib.snr_adam_step_dev(ptr(n.flat.data), ptr(gr), ptr(m), ptr(v), n.flat.numel(), ptr(G["state"]), 0.9, 0.999,
                                             1e-8, 1.0, _lib.stream()), "snr_adam_step_dev")
@@ -342,7 +362,7 @@ class RenderTrainer:
                                 'use_viewdirs') if not isinstance(kw.get(k), torch.Tensor))
         key = (H, W, float(focal), tuple(batch_rays.shape), str(batch_rays.device),
                tuple(n.flat.data_ptr() for n in self.nets), tuple(m.data_ptr() for m in self.m + self.v),
-               baked, float(self.lrate), float(self.lrate_decay),
+               baked, float(self.lrate), float(self.lrate_decay), tuple(sorted(self.muon.items())) if self.muon is not None else None,
                tuple(n.cfg.key() if hasattr(getattr(n, "cfg", None), "key") else None for n in self.nets))
         if self._graph is None or self._graph["key"] != key:
             if self._graph_warm != key:
@@ -579,14 +599,18 @@ class RenderTrainer:
     def state_dict(self):
         """{'global_step', 'network_fn_state_dict', 'network_fine_state_dict', 'optimizer_state_dict'} with the
         optimizer state laid out as torch.optim.Adam over the per-layer parameters in `grad_vars` order
-        (coarse net's parameters, then the fine net's: run_nerf.py:398-425) — loadable by the reference."""
+        (coarse net's parameters, then the fine net's: run_nerf.py:398-425) — loadable by the reference.  With muon the hidden
+        matrices' entries hold a momentum_buffer in place of the moments: only a trainer with muon resumes from it."""
         fn, fine = self.kw.get('network_fn'), self.kw.get('network_fine')
         state, idx = {}, 0
         for n, m, v in zip(self.nets, self.m, self.v):
+            hidden = n.hidden_matrices() if self.muon is not None else ()
             # param_views: the parameters the reference module registers (NeRF_RGB has no alpha_linear, helpers:183-185)
             for (k, mv), vv in zip(n.param_views(m).items(), n.param_views(v).values()):
                 state[idx] = {'step': torch.tensor(float(self.opt_step)), 'exp_avg': mv.detach().clone(),
                               'exp_avg_sq': vv.detach().clone()}
+                if k in hidden:      # (no exp_avg: an Adam that is handed this state fails instead of dividing by a second moment of zero)
+                    state[idx] = {'step': state[idx]['step'], 'momentum_buffer': state[idx]['exp_avg']}
                 idx += 1
         group = {'lr': self.current_lr(), 'betas': (0.9, 0.999), 'eps': 1e-8, 'weight_decay': 0, 'amsgrad': False,
                  'maximize': False, 'foreach': None, 'capturable': False, 'differentiable': False, 'fused': None,
@@ -612,7 +636,7 @@ class RenderTrainer:
         from .render import scatter_per_layer_adam
         for m, v in zip(self.m, self.v):
             m.zero_(); v.zero_()
-        steps = set(scatter_per_layer_adam(st, self.nets, list(zip(self.m, self.v)))) if st else set()
+        steps = set(scatter_per_layer_adam(st, self.nets, list(zip(self.m, self.v)), muon=self.muon is not None)) if st else set()
         steps.discard(0.0) if len(steps) > 1 else None      # (a network all of whose layers are idle carries no step count)
         if len(steps) > 1:
             raise RuntimeError(f"checkpoint parameters disagree on the Adam step count: {sorted(steps)}")
@@ -635,6 +659,19 @@ class RenderTrainer:
             return None
         torch.cuda.synchronize()
         return sum(a.elapsed_time(b) for a, b in self._comm_events) / self._comm_steps
+
+    def _muon_step(self, live, lr=0.0, state=None):
+        """muon_step_ on the hidden matrices of all networks and adam_step_multi_ on what lies between them: [(net, gradient, m, v)]"""
+        mats, rest = ([], [], []), ([], [], [], [])
+        for n, g, m, v in live:
+            for k, buf in enumerate((n.flat.data, g, m)):
+                a, b = n.split_hidden(buf)
+                mats[k].extend(a)
+                rest[k].extend(b)
+            rest[3].extend(n.split_hidden(v)[1])
+        scale = 1.0 / self.world_size
+        ops.muon_step_(*mats, lr, grad_scale=scale, state=state, **self.muon)
+        ops.adam_step_multi_(*rest, lr, max(1, self.opt_step), grad_scale=scale, state=state)
 
     def apply_gradients(self):
         if self._dist:
@@ -663,6 +700,11 @@ class RenderTrainer:
         lr = self._lr
         from .nerf import NeRF
         live = [(n, m, v) for n, m, v in zip(self.nets, self.m, self.v) if n.flat.grad is not None]   # torch.optim.Adam skips parameters without a gradient
+        if self.muon is not None:
+            self._muon_step([(n, n.flat.grad, m, v) for n, m, v in live], lr)
+            for n, _, _ in live:
+                n.mark_weights_changed()   # written through raw pointers
+            live = []
         fused = [t for t in live if type(t[0]) is NeRF and t[0].flat.is_cuda and os.environ.get("SNR_NO_ADAM_PACK") != "1"]
         done = []
         if fused:
