@@ -37,7 +37,9 @@ struct OrthIo {
   int64_t part;          // first partial sum (doubles)
 };
 struct OrthTable { int n; OrthGeom g[kOrthMax]; };
-struct OrthArgs {        // kernel arguments: a miss on them costs a microsecond, so the stack is found by one load (find_stack)
+// What the launches of a sequence share.  The first one has it as arguments and leaves a copy in the workspace for the others: 3.6 KB of
+// arguments make a launch 1.6 us longer, and a miss on them costs another microsecond, so the stack is found by one load (find_stack).
+struct OrthArgs {
   int sym0[kOrthMax], full0[kOrthMax], chunk0[kOrthMax], split0[kOrthMax];   // each stack's first workgroup: symmetric products, B Y,
                                                                              // reduction, split
   OrthTable t;
@@ -68,9 +70,9 @@ __host__ __device__ inline OrthPlanes orth_planes(int rp, int cp, bool split) {
 }
 
 // the stack a workgroup belongs to: its lanes look at every stack's first workgroup at once
-__device__ __forceinline__ int find_stack(const int* first, int n, int block) {
+__device__ __forceinline__ int find_stack(const int* first, int block) {   // (INT_MAX behind the last stack)
   const int lane = threadIdx.x & 63;
-  const bool mine = lane < n && block >= first[lane < n ? lane : 0];
+  const bool mine = lane < kOrthMax && block >= first[lane < kOrthMax ? lane : 0];
   return __builtin_amdgcn_readfirstlane(__popcll(__ballot(mine)) - 1);
 }
 
@@ -129,8 +131,13 @@ __device__ __forceinline__ double block_sum(double v) {
 
 // ---- 1. momentum (in place) and the partial sums of squares of the update, in 64 bits and in a fixed order ------------------
 // A pass over the input, bound by memory: 16 B a lane where its place allows.
-__global__ __launch_bounds__(256) void orth_reduce_kernel(OrthArgs a) {
-  const int s = find_stack(a.chunk0, a.t.n, blockIdx.x);
+__global__ __launch_bounds__(256) void orth_reduce_kernel(OrthArgs a, OrthArgs* copy) {
+  if (blockIdx.x == 0) {
+    static_assert(sizeof(OrthArgs) % 8 == 0, "copied as words");
+    const uint64_t* from = (const uint64_t*)__builtin_amdgcn_kernarg_segment_ptr();    // (the first argument)
+    for (int k = threadIdx.x; k < (int)(sizeof(OrthArgs) / 8); k += 256) ((uint64_t*)copy)[k] = from[k];
+  }
+  const int s = find_stack(a.chunk0, blockIdx.x);
   const OrthIo& io = a.io[s];
   const int k = blockIdx.x - a.chunk0[s], mat = k / io.nchunk, ch = k % io.nchunk;
   const int64_t count = (int64_t)io.m * io.n;
@@ -173,8 +180,9 @@ __global__ __launch_bounds__(256) void orth_reduce_kernel(OrthArgs a) {
 }
 
 // ---- 2. Y = scaled input (transposed where it is tall) as planes, zero in the padding --------------------------------------------
-__global__ __launch_bounds__(256) void orth_split_kernel(OrthArgs a) {
-  const int s = find_stack(a.split0, a.t.n, blockIdx.x);
+__global__ __launch_bounds__(256) void orth_split_kernel(const OrthArgs* __restrict__ args) {
+  const OrthArgs& a = *args;
+  const int s = find_stack(a.split0, blockIdx.x);
   const OrthIo& io = a.io[s];
   const OrthGeom& G = a.t.g[s];
   const int nti = G.rp / kPad, ntj = G.cp / kPad;
@@ -412,11 +420,13 @@ template <int BAND> __device__ __forceinline__ void sym_tile(int t, int n, int& 
 }
 
 template <int PHASE, bool last, class C>
-__global__ __launch_bounds__(C::NT) void orth_product_kernel(OrthArgs a, OrthOut o, float ca, float cb, float cc, int flip) {
+__global__ __launch_bounds__(C::NT) void orth_product_kernel(const OrthArgs* __restrict__ args, OrthOut o, float ca, float cb, float cc, int flip) {
+  const OrthArgs& a = *args;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int block = xcd_block();
-  const int s = find_stack(PHASE == kApply ? a.full0 : a.sym0, a.t.n, block);
-  const OrthGeom& G = a.t.g[s];
+  const int s = find_stack(PHASE == kApply ? a.full0 : a.sym0, block);
+  const OrthGeom G = a.t.g[s];
+  char* const ws = a.ws;
   const int nti = (G.rp + C::T - 1) / C::T;
   int mat, ti, tj;
   if (PHASE == kApply) {
@@ -429,7 +439,7 @@ __global__ __launch_bounds__(C::NT) void orth_product_kernel(OrthArgs a, OrthOut
     sym_tile<C::BAND>(k % per, nti, ti, tj);
   }
   const OrthPlanes P = orth_planes(G.rp, G.cp, C::SPLIT);
-  _Float16* W = (_Float16*)(a.ws + G.ws) + mat * P.total;
+  _Float16* W = (_Float16*)(ws + G.ws) + mat * P.total;
   const int64_t yh = flip ? P.h[1] : P.h[0], yl = flip ? P.l[1] : P.l[0];
   const int wi = (wave / C::WJ) * (C::T / C::WI), wj = (wave % C::WJ) * (C::T / C::WJ);
   f32x16 acc[C::TI][C::TJ] = {}, acl[C::SPLIT ? C::TI : 1][C::SPLIT ? C::TJ : 1] = {};
@@ -460,6 +470,15 @@ __global__ __launch_bounds__(C::NT) void orth_product_kernel(OrthArgs a, OrthOut
     }
   }
   const int n = K / C::BK;
+  // (one block a wave: what the epilogue adds to is read ahead of the products)
+  constexpr bool EARLY = C::TI * C::TJ == 1 && PHASE != kGram;
+  const int64_t ld_out = PHASE == kApply ? G.cp : G.rp;
+  Half16 eh = {}, el = {};
+  if (EARLY) {
+    const int64_t y = (int64_t)(ti * C::T + wi + (lane >> 1)) * ld_out + tj * C::T + wj + (lane & 1) * 16;
+    eh = load16(W + (PHASE == kPoly ? P.ah : yh) + y);
+    if (PHASE == kApply || C::SPLIT) el = load16(W + (PHASE == kPoly ? P.al : yl) + y);
+  }
   // Slice k's last 16 of K are multiplied behind the barrier that frees its buffer and shows slice k + 1, whose first fragments are
   // read under them; slice k + STAGES is fetched into the buffer at once.
   constexpr int KK = C::BK / 16;
@@ -520,14 +539,14 @@ __global__ __launch_bounds__(C::NT) void orth_product_kernel(OrthArgs a, OrthOut
       }
       wave_sync();
       float v[16];
-      const int64_t y = (int64_t)(i0 + row) * (PHASE == kApply ? G.cp : G.rp) + j0 + c0;
+      const int64_t y = (int64_t)(i0 + row) * ld_out + j0 + c0;
       if (PHASE == kGram) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[e] = blk[row][c0 + e] * (kAs / (kYs * kYs));
       } else {
-        const Half16 h = load16(W + (PHASE == kPoly ? P.ah : yh) + y);
-        Half16 l;
-        if (PHASE == kApply || C::SPLIT) l = load16(W + (PHASE == kPoly ? P.al : yl) + y);
+        const Half16 h = EARLY ? eh : load16(W + (PHASE == kPoly ? P.ah : yh) + y);
+        Half16 l = el;
+        if (!EARLY && (PHASE == kApply || C::SPLIT)) l = load16(W + (PHASE == kPoly ? P.al : yl) + y);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           float old = (float)(e < 8 ? h.a[e & 7] : h.b[e & 7]);
@@ -596,7 +615,7 @@ __global__ __launch_bounds__(256) void orth_small_kernel(OrthArgs a, OrthOut o, 
   constexpr int LD = 64 * NB + 8, LA = 64 + 8;       // rows in fp16: 16 B off a multiple of 128, so that 16 rows at one k spread over the banks
   __shared__ __attribute__((aligned(16))) _Float16 yh[64 * LD], yl[64 * LD], ah[64 * LA], al[64 * LA], bh[64 * LA], bl[64 * LA];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int s = find_stack(a.sym0, a.t.n, blockIdx.x);
+  const int s = find_stack(a.sym0, blockIdx.x);
   const OrthIo& io = a.io[s];
   const int64_t mat = blockIdx.x - a.sym0[s];
   const bool tall = io.m > io.n;
@@ -759,7 +778,7 @@ template <int PHASE> struct Largest { using Cfg = H192; };
 template <> struct Largest<kApply> { using Cfg = H256; };
 
 // Everything of a launch sequence that follows from its stacks' sizes; also the bytes of its workspace.
-struct OrthPlan { int ts, tf; int64_t sym, full, chunk, split, bytes; };
+struct OrthPlan { int ts, tf; int64_t sym, full, chunk, split, bytes; OrthArgs* args; };
 
 static int64_t sym_tiles(const OrthGeom& g, int T) { const int64_t t = (g.rp + T - 1) / T; return g.batch * (t * (t + 1) / 2); }
 static int64_t full_tiles(const OrthGeom& g, int T) { return (int64_t)g.batch * ((g.rp + T - 1) / T) * ((g.cp + T - 1) / T); }
@@ -780,6 +799,7 @@ static int orth_plan(OrthArgs& a, int kind, OrthPlan& p) {
   int64_t off = 0, part = 0;
   const bool split = kind != kHalf;
   p.chunk = p.split = p.sym = p.full = 0;
+  for (int s = a.t.n; s < kOrthMax; ++s) a.sym0[s] = a.full0[s] = a.chunk0[s] = a.split0[s] = INT32_MAX;
   if (kind < kSplit) {                       // a workgroup a matrix, no workspace
     for (int s = 0; s < a.t.n; ++s) { a.sym0[s] = (int)p.sym; p.sym += a.t.g[s].batch; }
     p.bytes = 256;
@@ -805,18 +825,20 @@ static int orth_plan(OrthArgs& a, int kind, OrthPlan& p) {
     p.sym += sym_tiles(a.t.g[s], p.ts); p.full += full_tiles(a.t.g[s], p.tf);
   }
   const int64_t at_part = align256(off);     // the planes come first: on 256 bytes
-  p.bytes = at_part + align256(part * 8);
+  const int64_t at_args = at_part + align256(part * 8);
+  p.args = (OrthArgs*)(a.ws + at_args);
+  p.bytes = at_args + align256(sizeof(OrthArgs));
   a.part = (double*)(a.ws + at_part);
   a.split = split;
   return SNR_OK;
 }
 
 template <int PHASE, bool last, class C>
-static void launch(const OrthArgs& a, const OrthOut& o, int64_t n, float ca, float cb, float cc, int flip, hipStream_t st) {
+static void launch(const OrthArgs* a, const OrthOut& o, int64_t n, float ca, float cb, float cc, int flip, hipStream_t st) {
   orth_product_kernel<PHASE, last, C><<<dim3((unsigned)n), dim3(C::NT), 0, st>>>(a, o, ca, cb, cc, flip);
 }
 template <int PHASE, bool last>
-static void launch_tile(bool split, int T, const OrthArgs& a, const OrthOut& o, int64_t n, float ca, float cb, float cc, int flip, hipStream_t st) {
+static void launch_tile(bool split, int T, const OrthArgs* a, const OrthOut& o, int64_t n, float ca, float cb, float cc, int flip, hipStream_t st) {
   if (split) {
     if (T == 64) launch<PHASE, last, S64>(a, o, n, ca, cb, cc, flip, st);
     else launch<PHASE, last, S128>(a, o, n, ca, cb, cc, flip, st);
@@ -849,15 +871,21 @@ static int orth_run(OrthArgs& a, const OrthOut& o, int steps, float ca, float cb
   }
   {
     ProfScope ps(K_ORTH_PREPARE, st);
-    orth_reduce_kernel<<<dim3((unsigned)p.chunk), dim3(256), 0, st>>>(a);
-    orth_split_kernel<<<dim3((unsigned)p.split), dim3(256), 0, st>>>(a);
+    orth_reduce_kernel<<<dim3((unsigned)p.chunk), dim3(256), 0, st>>>(a, p.args);
+    orth_split_kernel<<<dim3((unsigned)p.split), dim3(256), 0, st>>>(p.args);
   }
   for (int k = 0; k < steps; ++k) {
-    ProfScope ps(K_ORTH_PRODUCT, st);
-    launch_tile<kGram, false>(split, p.ts, a, o, p.sym, ca, cb, cc, k & 1, st);
-    launch_tile<kPoly, false>(split, p.ts, a, o, p.sym, ca, cb, cc, k & 1, st);
-    if (k + 1 == steps) launch_tile<kApply, true>(split, p.tf, a, o, p.full, ca, cb, cc, k & 1, st);
-    else launch_tile<kApply, false>(split, p.tf, a, o, p.full, ca, cb, cc, k & 1, st);
+    {
+      ProfScope ps(K_ORTH_GRAM, st);
+      launch_tile<kGram, false>(split, p.ts, p.args, o, p.sym, ca, cb, cc, k & 1, st);
+    }
+    {
+      ProfScope ps(K_ORTH_POLY, st);
+      launch_tile<kPoly, false>(split, p.ts, p.args, o, p.sym, ca, cb, cc, k & 1, st);
+    }
+    ProfScope ps(K_ORTH_APPLY, st);
+    if (k + 1 == steps) launch_tile<kApply, true>(split, p.tf, p.args, o, p.full, ca, cb, cc, k & 1, st);
+    else launch_tile<kApply, false>(split, p.tf, p.args, o, p.full, ca, cb, cc, k & 1, st);
   }
   return launch_status();
 }

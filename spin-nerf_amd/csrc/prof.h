@@ -10,7 +10,7 @@ enum KernelId {
   K_COMPOSITE_BWD, K_SAMPLE_FINE, K_MAKE_RAYS, K_ADAM, K_HG_PACK, K_HG_FWD, K_HG_BWD, K_MLP_WGRAD_PAIR,
   // (round 5) one id per kernel the training step launches, named like the kernel (bench.py's `kernels` keys = rocprofv3's names)
   K_COMPOSITE_TRAIN, K_COMPOSITE_TRAIN_REG, K_COMPOSITE_TRAIN_SAMPLE, K_PACK_RAYS_SAMPLE, K_PACK_RAYS, K_ADAM_PACK, K_WGRAD_POST,
-  K_ADAM_MULTI, K_ORTH_PREPARE, K_ORTH_PRODUCT, K_ORTH_SMALL,
+  K_ADAM_MULTI, K_ORTH_PREPARE, K_ORTH_GRAM, K_ORTH_POLY, K_ORTH_APPLY, K_ORTH_SMALL,
   K_COUNT
 };
 
