@@ -386,7 +386,7 @@ int snr_adam_pack_multi(const snr_adam_pack_item* items, int n_items, float lr, 
 /* Adam on a list of tensors in ONE launch (48 tensors a launch): the update of snr_adam_step, bit for bit, on ranges that do not
  * touch each other — what of a network is no hidden matrix (input layer, heads, biases) when snr_muon_step_multi takes the rest.
  * state NULL: rate `lr` and bias corrections from `step` (1-based); else both are read from the device-side snr_step_state.
- * Items with n == 0 are skipped. */
+ * Items with n == 0 are skipped; what is written must not share memory with anything else of the call (SNR_ERR_SHAPE). */
 typedef struct snr_adam_item {
   float* params;
   const float* grads;
@@ -414,8 +414,8 @@ int snr_orthogonalise(const void* x, int dtype, int64_t batch, int64_t rows, int
 /* The optimizer step around it, for a list of stacks (contiguous fp32 [batch, rows, cols]):
  *   momentum <- mu momentum + grad_scale g;   u = grad_scale g + mu momentum (nesterov) or momentum;
  *   params <- params (1 - lr weight_decay) - lr q orthogonalise(u)
- * q = 1, sqrt(max(1, rows / cols)) or 0.2 sqrt(max(rows, cols)) (SNR_MUON_NONE / _SPECTRAL / _RMS).  params and momentum of the
- * items must not overlap.  state: as above (only the rate is read). */
+ * q = 1, sqrt(max(1, rows / cols)) or 0.2 sqrt(max(rows, cols)) (SNR_MUON_NONE / _SPECTRAL / _RMS).  What is written must not share
+ * memory with anything else of the call (SNR_ERR_SHAPE).  state: as above (only the rate is read). */
 enum { SNR_MUON_NONE = 0, SNR_MUON_SPECTRAL = 1, SNR_MUON_RMS = 2 };
 typedef struct snr_muon_item {
   float* params;

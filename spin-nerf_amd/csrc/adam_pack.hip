@@ -356,6 +356,16 @@ extern "C" int snr_adam_step_multi(const snr_adam_item* items, int n_items, floa
     SNR_CHECK_ARG(items[i].n >= 0 && items[i].n <= (int64_t)1 << 40, SNR_ERR_SHAPE);
     SNR_CHECK_ARG(items[i].n == 0 || (items[i].params && items[i].grads && items[i].exp_avg && items[i].exp_avg_sq), SNR_ERR_NULL);
   }
+  Span* spans = (Span*)malloc(sizeof(Span) * 4 * (size_t)n_items);
+  if (!spans) return (int)hipErrorOutOfMemory;
+  for (int i = 0; i < n_items; ++i) {
+    const snr_adam_item& it = items[i];
+    const void* at[4] = {it.params, it.grads, it.exp_avg, it.exp_avg_sq};
+    for (int k = 0; k < 4; ++k) spans[4 * i + k] = Span{(uintptr_t)at[k], (uintptr_t)at[k] + 4 * (uintptr_t)it.n, k != 1};
+  }
+  const bool clash = spans_clash(spans, 4 * (size_t)n_items);
+  free(spans);
+  SNR_CHECK_ARG(!clash, SNR_ERR_SHAPE);
   const float bc1 = state ? 1.f : (float)(1.0 - powi_host((double)beta1, step));
   const float bc2_sqrt = state ? 1.f : (float)sqrt(1.0 - powi_host((double)beta2, step));
   for (int i = 0; i < n_items;) {

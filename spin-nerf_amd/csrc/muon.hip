@@ -17,38 +17,49 @@
 
 namespace snr {
 
-constexpr int kOrthMax = 24;                // stacks per launch sequence: the kernel arguments hold the table
+constexpr int kOrthMax = 24;                // items per launch sequence: the first kernel's arguments hold the table
 constexpr int kPad = 64;                    // what the planes' sides are padded to
 constexpr float kYs = 1024.f, kAs = 512.f;  // powers of two that the planes of Y and of A, B are scaled by
 constexpr float kLo = 2048.f;               // ... and the lo planes on top
 
-struct OrthGeom {        // a stack of equal matrices
+struct OrthGeom {        // matrices of one size, whatever items they come from
   int r, c, rp, cp;      // sides of Y, and padded
-  int batch;
-  int64_t ws;            // its planes
+  int batch, pad;
+  int64_t ws;            // their planes
 };
-struct OrthIo {
+struct OrthIo {          // an item: a stack of matrices
   const void* x;         // the input, or the gradients
   void* out;             // the result, or the parameters
   float* mom;            // momentum (null: plain orthogonalisation)
   int64_t xb, xr, ob, orow;  // element strides: matrix, row (columns are contiguous)
   int m, n;              // sizes as stored
+  int batch, geom, mat0; // its matrices are those of a geometry from mat0 on
   int nchunk;            // workgroups (partial sums) per matrix in the reduction
   int64_t part;          // first partial sum (doubles)
 };
-struct OrthTable { int n; OrthGeom g[kOrthMax]; };
 // What the launches of a sequence share.  The first one has it as arguments and leaves a copy in the workspace for the others: 3.6 KB of
-// arguments make a launch 1.6 us longer, and a miss on them costs another microsecond, so the stack is found by one load (find_stack).
+// arguments make a launch 1.6 us longer, and a miss on them costs another microsecond, so an item is found by one load (find_item).
 struct OrthArgs {
-  int sym0[kOrthMax], full0[kOrthMax], chunk0[kOrthMax], split0[kOrthMax];   // each stack's first workgroup: symmetric products, B Y,
-                                                                             // reduction, split
-  OrthTable t;
+  int chunk0[kOrthMax], split0[kOrthMax];   // each item's first workgroup in the reduction and in the split
+  int sym0[kOrthMax], full0[kOrthMax];      // each geometry's in the symmetric products and in B Y (small kernel: each item's in sym0)
+  int n_geom, n_items;
+  OrthGeom g[kOrthMax];
   OrthIo io[kOrthMax];
   int dtype;             // of x / out without momentum
   float mu, gscale, eps;
   int nesterov, split;
   double* part;
   char* ws;
+};
+// What a product needs of it, as arguments where there are few geometries: no chain of loads before the first slice is asked for.
+constexpr int kHead = 4;
+struct OrthHead {
+  const OrthArgs* args;
+  char* ws;
+  int n;                 // 0: look them up in args
+  int first[kHead];      // of the phase
+  int pad;
+  OrthGeom g[kHead];
 };
 struct OrthOut {         // the last product's epilogue
   int dtype, muon, scale_mode;
@@ -69,8 +80,8 @@ __host__ __device__ inline OrthPlanes orth_planes(int rp, int cp, bool split) {
   return p;
 }
 
-// the stack a workgroup belongs to: its lanes look at every stack's first workgroup at once
-__device__ __forceinline__ int find_stack(const int* first, int block) {   // (INT_MAX behind the last stack)
+// the item (geometry) a workgroup belongs to: its lanes look at every one's first workgroup at once
+__device__ __forceinline__ int find_item(const int* first, int block) {   // (INT_MAX behind the last)
   const int lane = threadIdx.x & 63;
   const bool mine = lane < kOrthMax && block >= first[lane < kOrthMax ? lane : 0];
   return __builtin_amdgcn_readfirstlane(__popcll(__ballot(mine)) - 1);
@@ -137,7 +148,7 @@ __global__ __launch_bounds__(256) void orth_reduce_kernel(OrthArgs a, OrthArgs* 
     const uint64_t* from = (const uint64_t*)__builtin_amdgcn_kernarg_segment_ptr();    // (the first argument)
     for (int k = threadIdx.x; k < (int)(sizeof(OrthArgs) / 8); k += 256) ((uint64_t*)copy)[k] = from[k];
   }
-  const int s = find_stack(a.chunk0, blockIdx.x);
+  const int s = find_item(a.chunk0, blockIdx.x);
   const OrthIo& io = a.io[s];
   const int k = blockIdx.x - a.chunk0[s], mat = k / io.nchunk, ch = k % io.nchunk;
   const int64_t count = (int64_t)io.m * io.n;
@@ -182,9 +193,9 @@ __global__ __launch_bounds__(256) void orth_reduce_kernel(OrthArgs a, OrthArgs* 
 // ---- 2. Y = scaled input (transposed where it is tall) as planes, zero in the padding --------------------------------------------
 __global__ __launch_bounds__(256) void orth_split_kernel(const OrthArgs* __restrict__ args) {
   const OrthArgs& a = *args;
-  const int s = find_stack(a.split0, blockIdx.x);
+  const int s = find_item(a.split0, blockIdx.x);
   const OrthIo& io = a.io[s];
-  const OrthGeom& G = a.t.g[s];
+  const OrthGeom& G = a.g[io.geom];
   const int nti = G.rp / kPad, ntj = G.cp / kPad;
   const int k = blockIdx.x - a.split0[s], mat = k / (nti * ntj), t = k % (nti * ntj);
   const int i0 = t / ntj * kPad, j0 = t % ntj * kPad;
@@ -195,7 +206,7 @@ __global__ __launch_bounds__(256) void orth_split_kernel(const OrthArgs* __restr
   const double norm = sqrt(block_sum(sum));
   const double scale = (double)kYs / (norm < (double)a.eps ? (double)a.eps : norm);   // (a NaN stays one)
   const OrthPlanes P = orth_planes(G.rp, G.cp, a.split);
-  _Float16* W = (_Float16*)(a.ws + G.ws) + mat * P.total;
+  _Float16* W = (_Float16*)(a.ws + G.ws) + (io.mat0 + mat) * P.total;
   typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
   // four columns a thread, sixteen rows of the input at once
   const int b = io.mom ? 4 : type_bytes(a.dtype);
@@ -420,26 +431,41 @@ template <int BAND> __device__ __forceinline__ void sym_tile(int t, int n, int& 
 }
 
 template <int PHASE, bool last, class C>
-__global__ __launch_bounds__(C::NT) void orth_product_kernel(const OrthArgs* __restrict__ args, OrthOut o, float ca, float cb, float cc, int flip) {
-  const OrthArgs& a = *args;
+__global__ __launch_bounds__(C::NT) void orth_product_kernel(OrthHead h, OrthOut o, float ca, float cb, float cc, int flip) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int block = xcd_block();
-  const int s = find_stack(PHASE == kApply ? a.full0 : a.sym0, block);
-  const OrthGeom G = a.t.g[s];
-  char* const ws = a.ws;
+  // (asked for together: one after the other they are a miss each)
+  asm volatile("" ::"s"(h.n), "s"(h.ws), "s"(h.first[1]), "s"(h.first[2]), "s"(h.first[3]), "s"(h.g[0].rp), "s"(h.g[0].cp), "s"(h.g[0].ws),
+               "s"(h.g[1].rp), "s"(h.g[1].ws), "s"(h.g[2].rp), "s"(h.g[2].ws), "s"(h.g[3].rp), "s"(h.g[3].ws));
+  int s = 0, first = 0;
+  struct { int r, c, rp, cp; int64_t ws; } G = {h.g[0].r, h.g[0].c, h.g[0].rp, h.g[0].cp, h.g[0].ws};
+  if (h.n == 0) {
+    const int* const all = PHASE == kApply ? h.args->full0 : h.args->sym0;
+    s = find_item(all, block); first = all[s];
+    const OrthGeom& g = h.args->g[s];
+    G.r = g.r; G.c = g.c; G.rp = g.rp; G.cp = g.cp; G.ws = g.ws;
+  } else {
+#pragma unroll
+    for (int k = 1; k < kHead; ++k) {
+      const bool is = block >= h.first[k];
+      s = is ? k : s; first = is ? h.first[k] : first;
+      G.r = is ? h.g[k].r : G.r; G.c = is ? h.g[k].c : G.c; G.rp = is ? h.g[k].rp : G.rp; G.cp = is ? h.g[k].cp : G.cp;
+      G.ws = is ? h.g[k].ws : G.ws;
+    }
+  }
   const int nti = (G.rp + C::T - 1) / C::T;
   int mat, ti, tj;
   if (PHASE == kApply) {
-    const int ntj = (G.cp + C::T - 1) / C::T, k = block - a.full0[s], t = k % (nti * ntj), band = t / (C::BAND * ntj);
+    const int ntj = (G.cp + C::T - 1) / C::T, k = block - first, t = k % (nti * ntj), band = t / (C::BAND * ntj);
     const int h = nti - band * C::BAND < C::BAND ? nti - band * C::BAND : C::BAND, q = t - band * C::BAND * ntj;
     mat = k / (nti * ntj); ti = band * C::BAND + q % h; tj = q / h;
   } else {
-    const int per = nti * (nti + 1) / 2, k = block - a.sym0[s];
+    const int per = nti * (nti + 1) / 2, k = block - first;
     mat = k / per;
     sym_tile<C::BAND>(k % per, nti, ti, tj);
   }
   const OrthPlanes P = orth_planes(G.rp, G.cp, C::SPLIT);
-  _Float16* W = (_Float16*)(ws + G.ws) + mat * P.total;
+  _Float16* W = (_Float16*)(h.ws + G.ws) + mat * P.total;
   const int64_t yh = flip ? P.h[1] : P.h[0], yl = flip ? P.l[1] : P.l[0];
   const int wi = (wave / C::WJ) * (C::T / C::WI), wj = (wave % C::WJ) * (C::T / C::WJ);
   f32x16 acc[C::TI][C::TJ] = {}, acl[C::SPLIT ? C::TI : 1][C::SPLIT ? C::TJ : 1] = {};
@@ -519,9 +545,17 @@ __global__ __launch_bounds__(C::NT) void orth_product_kernel(const OrthArgs* __r
   // 32 B a lane
   float (*blk)[36] = (float (*)[36])(s0 + wave * (32 * 36 * 4));
   float lr_q = 0.f, keep = 1.f;
-  if (PHASE == kApply && last) muon_rate(o, a.io[s], lr_q, keep);
+  int item = 0;
+  if (last) {                         // the item that the matrix belongs to, and its number there
+    const OrthArgs& a = *h.args;
+    const int at = lane < kOrthMax ? lane : 0;
+    const bool mine = lane < a.n_items && a.io[at].geom == s && mat >= a.io[at].mat0 && mat < a.io[at].mat0 + a.io[at].batch;
+    item = __builtin_amdgcn_readfirstlane(__ffsll(__ballot(mine)) - 1);
+    mat -= a.io[item].mat0;
+    muon_rate(o, a.io[item], lr_q, keep);
+  }
+  const OrthIo& io = h.args->io[item];
   const int row = lane >> 1, c0 = (lane & 1) * 16;
-  const OrthIo& io = a.io[s];
   bool wide = false;                  // 16-byte pieces of the result
   if (last) { const int b = o.muon ? 4 : type_bytes(o.dtype); wide = on_grid(io.out, mat * io.ob * b, io.orow * b, 16); }
 #pragma unroll
@@ -615,7 +649,7 @@ __global__ __launch_bounds__(256) void orth_small_kernel(OrthArgs a, OrthOut o, 
   constexpr int LD = 64 * NB + 8, LA = 64 + 8;       // rows in fp16: 16 B off a multiple of 128, so that 16 rows at one k spread over the banks
   __shared__ __attribute__((aligned(16))) _Float16 yh[64 * LD], yl[64 * LD], ah[64 * LA], al[64 * LA], bh[64 * LA], bl[64 * LA];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int s = find_stack(a.sym0, blockIdx.x);
+  const int s = find_item(a.sym0, blockIdx.x);
   const OrthIo& io = a.io[s];
   const int64_t mat = blockIdx.x - a.sym0[s];
   const bool tall = io.m > io.n;
@@ -789,7 +823,7 @@ static int64_t full_tiles(const OrthGeom& g, int T) { return (int64_t)g.batch * 
 // 2 of 1024 x 4096: 55 / 47 / 62 / 55.  fp32 (no larger tile fits LDS twice), 2048^2: 53 / 54, 67 / 65; 14 x 256^2: 7 / 13.
 template <class F> static int pick_tile(const OrthArgs& a, bool split, int largest, F tiles) {
   int64_t n[2] = {0, 0};
-  for (int s = 0; s < a.t.n; ++s) { n[0] += tiles(a.t.g[s], largest); n[1] += tiles(a.t.g[s], 128); }
+  for (int s = 0; s < a.n_geom; ++s) { n[0] += tiles(a.g[s], largest); n[1] += tiles(a.g[s], 128); }
   const int cus = cu_count();
   if (!split && n[0] >= cus * 3 / 4) return largest;
   return n[1] >= cus / 2 ? 128 : 64;
@@ -799,46 +833,59 @@ static int orth_plan(OrthArgs& a, int kind, OrthPlan& p) {
   int64_t off = 0, part = 0;
   const bool split = kind != kHalf;
   p.chunk = p.split = p.sym = p.full = 0;
-  for (int s = a.t.n; s < kOrthMax; ++s) a.sym0[s] = a.full0[s] = a.chunk0[s] = a.split0[s] = INT32_MAX;
+  for (int s = 0; s < kOrthMax; ++s) a.sym0[s] = a.full0[s] = a.chunk0[s] = a.split0[s] = INT32_MAX;
   if (kind < kSplit) {                       // a workgroup a matrix, no workspace
-    for (int s = 0; s < a.t.n; ++s) { a.sym0[s] = (int)p.sym; p.sym += a.t.g[s].batch; }
+    for (int s = 0; s < a.n_items; ++s) { a.sym0[s] = (int)p.sym; p.sym += a.io[s].batch; }
     p.bytes = 256;
     return SNR_OK;
   }
-  for (int s = 0; s < a.t.n; ++s) {
+  a.n_geom = 0;
+  for (int s = 0; s < a.n_items; ++s) {
     OrthIo& io = a.io[s];
-    OrthGeom& g = a.t.g[s];
-    g.r = io.m < io.n ? io.m : io.n; g.c = io.m < io.n ? io.n : io.m;
-    g.rp = (g.r + kPad - 1) / kPad * kPad; g.cp = (g.c + kPad - 1) / kPad * kPad;
+    const int r = io.m < io.n ? io.m : io.n, c = io.m < io.n ? io.n : io.m;
+    int k = 0;
+    while (k < a.n_geom && (a.g[k].r != r || a.g[k].c != c)) ++k;
+    if (k == a.n_geom) a.g[a.n_geom++] = OrthGeom{r, c, (r + kPad - 1) / kPad * kPad, (c + kPad - 1) / kPad * kPad, 0, 0, 0};
+    OrthGeom& g = a.g[k];
+    io.geom = k; io.mat0 = g.batch; g.batch += io.batch;
     const int64_t n = ((int64_t)io.m * io.n + 8191) / 8192;
     io.nchunk = (int)(n > 1024 ? 1024 : n);
-    io.part = part; part += (int64_t)g.batch * io.nchunk;
-    a.chunk0[s] = (int)p.chunk; p.chunk += (int64_t)g.batch * io.nchunk;
-    a.split0[s] = (int)p.split; p.split += (int64_t)g.batch * (g.rp / kPad) * (g.cp / kPad);
-    g.ws = off; off += (int64_t)g.batch * orth_planes(g.rp, g.cp, split).total * 2;
+    io.part = part; part += (int64_t)io.batch * io.nchunk;
+    a.chunk0[s] = (int)p.chunk; p.chunk += (int64_t)io.batch * io.nchunk;
+    a.split0[s] = (int)p.split; p.split += (int64_t)io.batch * (g.rp / kPad) * (g.cp / kPad);
     if (p.chunk > INT32_MAX || p.split > INT32_MAX) return SNR_ERR_SHAPE;
   }
   p.ts = pick_tile(a, split, 192, sym_tiles);
   p.tf = pick_tile(a, split, 256, full_tiles);
-  for (int s = 0; s < a.t.n; ++s) {          // (no more than the split's: a tile holds 64 x 64 or more)
+  for (int s = 0; s < a.n_geom; ++s) {       // (no more tiles than the split's: one holds 64 x 64 or more)
+    OrthGeom& g = a.g[s];
+    g.ws = off; off += (int64_t)g.batch * orth_planes(g.rp, g.cp, split).total * 2;
     a.sym0[s] = (int)p.sym; a.full0[s] = (int)p.full;
-    p.sym += sym_tiles(a.t.g[s], p.ts); p.full += full_tiles(a.t.g[s], p.tf);
+    p.sym += sym_tiles(g, p.ts); p.full += full_tiles(g, p.tf);
   }
   const int64_t at_part = align256(off);     // the planes come first: on 256 bytes
+  a.part = (double*)(a.ws + at_part);
+  a.split = split;
   const int64_t at_args = at_part + align256(part * 8);
   p.args = (OrthArgs*)(a.ws + at_args);
   p.bytes = at_args + align256(sizeof(OrthArgs));
-  a.part = (double*)(a.ws + at_part);
-  a.split = split;
   return SNR_OK;
 }
 
+static OrthHead orth_head(const OrthArgs& a, const OrthArgs* in_ws, const int* first) {
+  OrthHead h{};
+  h.args = in_ws; h.ws = a.ws;
+  h.n = a.n_geom <= kHead ? a.n_geom : 0;
+  for (int k = 0; k < kHead; ++k) { h.first[k] = k < a.n_geom ? first[k] : INT32_MAX; h.g[k] = a.g[k]; }
+  return h;
+}
+
 template <int PHASE, bool last, class C>
-static void launch(const OrthArgs* a, const OrthOut& o, int64_t n, float ca, float cb, float cc, int flip, hipStream_t st) {
+static void launch(const OrthHead& a, const OrthOut& o, int64_t n, float ca, float cb, float cc, int flip, hipStream_t st) {
   orth_product_kernel<PHASE, last, C><<<dim3((unsigned)n), dim3(C::NT), 0, st>>>(a, o, ca, cb, cc, flip);
 }
 template <int PHASE, bool last>
-static void launch_tile(bool split, int T, const OrthArgs* a, const OrthOut& o, int64_t n, float ca, float cb, float cc, int flip, hipStream_t st) {
+static void launch_tile(bool split, int T, const OrthHead& a, const OrthOut& o, int64_t n, float ca, float cb, float cc, int flip, hipStream_t st) {
   if (split) {
     if (T == 64) launch<PHASE, last, S64>(a, o, n, ca, cb, cc, flip, st);
     else launch<PHASE, last, S128>(a, o, n, ca, cb, cc, flip, st);
@@ -851,7 +898,7 @@ static void launch_tile(bool split, int T, const OrthArgs* a, const OrthOut& o, 
   }
 }
 
-// one launch sequence over a.t.n stacks of one precision whose io fields x, out, mom, strides, m, n and g.batch are filled in
+// one launch sequence over a.n_items items of one kind, whose x, out, mom, strides, m, n and batch are filled in
 static int orth_run(OrthArgs& a, const OrthOut& o, int steps, float ca, float cb, float cc, int kind, char* ws, hipStream_t st) {
   a.ws = ws;
   OrthPlan p;
@@ -874,18 +921,19 @@ static int orth_run(OrthArgs& a, const OrthOut& o, int steps, float ca, float cb
     orth_reduce_kernel<<<dim3((unsigned)p.chunk), dim3(256), 0, st>>>(a, p.args);
     orth_split_kernel<<<dim3((unsigned)p.split), dim3(256), 0, st>>>(p.args);
   }
+  const OrthHead hs = orth_head(a, p.args, a.sym0), hf = orth_head(a, p.args, a.full0);
   for (int k = 0; k < steps; ++k) {
     {
       ProfScope ps(K_ORTH_GRAM, st);
-      launch_tile<kGram, false>(split, p.ts, p.args, o, p.sym, ca, cb, cc, k & 1, st);
+      launch_tile<kGram, false>(split, p.ts, hs, o, p.sym, ca, cb, cc, k & 1, st);
     }
     {
       ProfScope ps(K_ORTH_POLY, st);
-      launch_tile<kPoly, false>(split, p.ts, p.args, o, p.sym, ca, cb, cc, k & 1, st);
+      launch_tile<kPoly, false>(split, p.ts, hs, o, p.sym, ca, cb, cc, k & 1, st);
     }
     ProfScope ps(K_ORTH_APPLY, st);
-    if (k + 1 == steps) launch_tile<kApply, true>(split, p.tf, p.args, o, p.full, ca, cb, cc, k & 1, st);
-    else launch_tile<kApply, false>(split, p.tf, p.args, o, p.full, ca, cb, cc, k & 1, st);
+    if (k + 1 == steps) launch_tile<kApply, true>(split, p.tf, hf, o, p.full, ca, cb, cc, k & 1, st);
+    else launch_tile<kApply, false>(split, p.tf, hf, o, p.full, ca, cb, cc, k & 1, st);
   }
   return launch_status();
 }
@@ -896,7 +944,7 @@ extern "C" int64_t snr_orthogonalise_ws_bytes(int64_t batch, int64_t rows, int64
   if (st != SNR_OK) return st;
   OrthArgs A{};
   OrthPlan p;
-  A.t.n = 1; A.t.g[0].batch = (int)batch; A.io[0].m = (int)rows; A.io[0].n = (int)cols;
+  A.n_items = 1; A.io[0].batch = (int)batch; A.io[0].m = (int)rows; A.io[0].n = (int)cols;
   const int ok = orth_plan(A, kind_of(precision, rows, cols), p);
   return ok != SNR_OK ? ok : p.bytes;
 }
@@ -911,8 +959,8 @@ extern "C" int snr_orthogonalise(const void* x, int dtype, int64_t batch, int64_
   SNR_CHECK_ARG(precision == SNR_ORTH_FP16 || precision == SNR_ORTH_FP32, SNR_ERR_UNSUPPORTED);
   SNR_CHECK_ARG(orth_bounded(steps, a, b, c), SNR_ERR_UNSUPPORTED);
   OrthArgs A{};
-  A.t.n = 1; A.t.g[0].batch = (int)batch;
-  A.io[0] = OrthIo{x, out, nullptr, x_batch_stride, x_row_stride, out_batch_stride, out_row_stride, (int)rows, (int)cols, 0, 0};
+  A.n_items = 1;
+  A.io[0] = OrthIo{x, out, nullptr, x_batch_stride, x_row_stride, out_batch_stride, out_row_stride, (int)rows, (int)cols, (int)batch, 0, 0, 0, 0};
   A.dtype = dtype; A.eps = eps;
   OrthOut o{};
   o.dtype = dtype;
@@ -925,17 +973,16 @@ template <class F> static int for_sequences(const snr_muon_item* items, int n_it
   for (int kind = 0; kind < kKinds; ++kind) {
     OrthArgs A{};
     for (int i = 0; i <= n_items; ++i) {
-      if (A.t.n == kOrthMax || (i == n_items && A.t.n)) {
+      if (A.n_items == kOrthMax || (i == n_items && A.n_items)) {
         const int st = f(A, kind);
         if (st != SNR_OK) return st;
-        A.t.n = 0;
+        A.n_items = 0;
       }
       if (i == n_items) break;
       const snr_muon_item& it = items[i];
       if (kind_of(precision, it.rows, it.cols) != kind) continue;
       const int64_t mn = it.rows * it.cols;
-      A.t.g[A.t.n].batch = (int)it.batch;
-      A.io[A.t.n++] = OrthIo{it.grads, it.params, it.momentum, mn, it.cols, mn, it.cols, (int)it.rows, (int)it.cols, 0, 0};
+      A.io[A.n_items++] = OrthIo{it.grads, it.params, it.momentum, mn, it.cols, mn, it.cols, (int)it.rows, (int)it.cols, (int)it.batch, 0, 0, 0, 0};
     }
   }
   return SNR_OK;
@@ -971,6 +1018,17 @@ extern "C" int snr_muon_step_multi(const snr_muon_item* items, int n_items, floa
     SNR_CHECK_ARG(items[i].params && items[i].grads && items[i].momentum, SNR_ERR_NULL);
     SNR_CHECK_ARG(stack_ok(items[i].batch, items[i].rows, items[i].cols) == SNR_OK, SNR_ERR_SHAPE);
   }
+  Span* spans = (Span*)malloc(sizeof(Span) * 3 * (size_t)n_items);
+  if (!spans) return (int)hipErrorOutOfMemory;
+  for (int i = 0; i < n_items; ++i) {
+    const snr_muon_item& it = items[i];
+    const void* at[3] = {it.params, it.grads, it.momentum};
+    const uintptr_t bytes = 4 * (uintptr_t)(it.batch * it.rows * it.cols);
+    for (int k = 0; k < 3; ++k) spans[3 * i + k] = Span{(uintptr_t)at[k], (uintptr_t)at[k] + bytes, k != 1};
+  }
+  const bool clash = spans_clash(spans, 3 * (size_t)n_items);
+  free(spans);
+  SNR_CHECK_ARG(!clash, SNR_ERR_SHAPE);
   OrthOut o{};
   o.muon = 1; o.scale_mode = scale_mode; o.lr = lr; o.decay = weight_decay; o.st = state;
   return for_sequences(items, n_items, precision, [&](OrthArgs& A, int kind) {

@@ -4,6 +4,7 @@
 #include <stdint.h>
 #include <stdlib.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "../../include/spinnerf_hip.h"
@@ -30,6 +31,20 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 inline int launch_status() {
   hipError_t e = hipGetLastError();
   return e == hipSuccess ? SNR_OK : (int)e;
+}
+
+// Whether a range that a launch writes touches another of its ranges: the items of a list are worked on side by side.
+struct Span { uintptr_t a, b; bool written; };
+inline bool spans_clash(Span* s, size_t n) {
+  std::sort(s, s + n, [](const Span& x, const Span& y) { return x.a < y.a; });
+  uintptr_t end_written = 0, end_any = 0;
+  for (size_t i = 0; i < n; ++i) {
+    if (s[i].a == s[i].b) continue;
+    if (s[i].a < (s[i].written ? end_any : end_written)) return true;
+    end_any = s[i].b > end_any ? s[i].b : end_any;
+    if (s[i].written && s[i].b > end_written) end_written = s[i].b;
+  }
+  return false;
 }
 
 // hipFuncAttributeMaxDynamicSharedMemorySize is a per-DEVICE property of a kernel: set it once per (kernel, device),

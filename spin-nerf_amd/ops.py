@@ -647,30 +647,60 @@ def adam_pack_step_(nets, grads, exp_avgs, exp_avg_sqs, lr, step, beta1=0.9, bet
     return True
 
 
-def _flat_list(name, params, *others):
-    """the tensors of an in-place optimizer call as lists: fp32, contiguous, on one device, equal sizes item by item, and no two
-    of the tensors that are written sharing memory (the items of a launch run side by side)"""
-    lists = [list(params)] + [list(o) for o in others]
+class _on:
+    """the device that a call's tensors live on, for the launches inside; nothing where it is the current one already"""
+
+    def __init__(self, index):
+        self.ctx = torch.cuda.device(index) if index != torch.cuda.current_device() else None
+
+    def __enter__(self):
+        if self.ctx is not None:
+            self.ctx.__enter__()
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+
+
+def _rows(name, lists, read):
+    """the lists of an in-place optimizer call row by row (tensors of one item): fp32, of one shape, on one device, contiguous; list
+    number ``read`` is only read, and copied where it is not contiguous.  Returns (rows, device index)."""
+    lists = [list(x) for x in lists]
     if any(len(x) != len(lists[0]) for x in lists):
         raise ValueError(f"{name}: the lists differ in length: {[len(x) for x in lists]}")
-    dev = None
-    for row in zip(*lists):
-        for t in row:
-            if not t.is_cuda:
-                raise _lib.HipLibraryError(f"{name}: the kernels need device (HIP) tensors; got a CPU tensor")
-            dev = t.device if dev is None else dev
-            if t.device != dev:
-                raise ValueError(f"{name}: expected a tensor on {dev}, got {t.device}")
+    rows, dev = list(zip(*lists)), None
+    for i, row in enumerate(rows):
+        first = row[0]
+        shape = first.shape
+        for k, t in enumerate(row):
+            at = t.get_device()
+            if at != dev:
+                if at < 0:
+                    raise _lib.HipLibraryError(f"{name}: the kernels need device (HIP) tensors; got a CPU tensor")
+                if dev is not None:
+                    raise ValueError(f"{name}: expected a tensor on cuda:{dev}, got {t.device}")
+                dev = at
             if t.dtype != torch.float32:
                 raise ValueError(f"{name}: expected float32, got {t.dtype}")
-            if t.shape != row[0].shape:
+            if t is not first and t.shape != shape:
                 raise ValueError(f"{name}: shapes of one item differ: {[tuple(u.shape) for u in row]}")
-    return lists, dev
+            if not t.is_contiguous():
+                if k != read:
+                    raise ValueError(f"{name}: tensors that are written must be contiguous; got strides {t.stride()} for {tuple(t.shape)}")
+                rows[i] = rows[i][:k] + (t.contiguous(),) + rows[i][k + 1:]
+    return rows, dev
 
 
-def _no_overlap(name, read, written):
-    """no tensor of ``written`` shares memory with another of ``written`` or with one of ``read``"""
-    spans = sorted([(t.data_ptr(), t.data_ptr() + 4 * t.numel(), w) for ts, w in ((written, True), (read, False)) for t in ts if t.numel()])
+def _items(struct, values):
+    """an array of a C struct whose fields are all 8 bytes, from them one after the other"""
+    import ctypes
+    flat = (ctypes.c_int64 * len(values))(*values)
+    return (struct * (len(values) // len(struct._fields_))).from_buffer(flat)
+
+
+def _no_overlap(name, rows, read):
+    """raises where a tensor that is written shares memory with another of the call (the library has found one that does)"""
+    spans = sorted((t.data_ptr(), t.data_ptr() + 4 * t.numel(), k != read) for row in rows for k, t in enumerate(row) if t.numel())
     end_w = end_any = 0
     for a, b, w in spans:
         if a < (end_any if w else end_w):
@@ -680,28 +710,21 @@ def _no_overlap(name, read, written):
             end_w = max(end_w, b)
 
 
-def _written(name, ts):
-    for t in ts:
-        if not t.is_contiguous():
-            raise ValueError(f"{name}: tensors that are written must be contiguous; got strides {t.stride()} for {tuple(t.shape)}")
-
-
 def adam_step_multi_(params, grads, exp_avgs, exp_avg_sqs, lr, step, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, state=None):
     """adam_step_ (bit for bit) on lists of fp32 tensors of any sizes in one launch per 48 tensors (snr_adam_step_multi): what of a
     network is no hidden matrix when muon_step_ takes the rest.  ``state``: a device-side snr_step_state whose rate and bias
     corrections count instead of ``lr`` and ``step`` (captured graphs)."""
-    (params, grads, ms, vs), dev = _flat_list("adam_step_multi_", params, grads, exp_avgs, exp_avg_sqs)
-    if not params:
+    rows, dev = _rows("adam_step_multi_", (params, grads, exp_avgs, exp_avg_sqs), 1)
+    if not rows:
         return
-    _written("adam_step_multi_", params + ms + vs)
-    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
-    _no_overlap("adam_step_multi_", grads, params + ms + vs)
     lib = _lib.load()
-    items = (_lib.AdamItem * len(params))(*[(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel())
-                                            for p, g, m, v in zip(params, grads, ms, vs)])
-    with torch.cuda.device(dev):
-        check(lib.snr_adam_step_multi(items, len(params), float(lr), float(beta1), float(beta2), float(eps), int(step), float(grad_scale),
-                                      ptr(state), stream()), "snr_adam_step_multi")
+    items = _items(_lib.AdamItem, [x for p, g, m, v in rows for x in (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel())])
+    with _on(dev):
+        st = lib.snr_adam_step_multi(items, len(rows), float(lr), float(beta1), float(beta2), float(eps), int(step), float(grad_scale),
+                                     ptr(state), stream())
+    if st:
+        _no_overlap("adam_step_multi_", rows, 1)
+        check(st, "snr_adam_step_multi")
 
 
 # ----------------------------------------------------------------------------------------------
@@ -764,7 +787,7 @@ def orthogonalise(x, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, precision=No
             y = y.clone()
         lib = _lib.load()
         dt, st, prec = _ORTH_TYPES[x.dtype], args[:5], args[5]
-        with torch.cuda.device(x.device):
+        with _on(x.get_device()):
             nbytes = lib.snr_orthogonalise_ws_bytes(y.shape[0], m, n, prec)
             if nbytes <= 0:
                 check(int(nbytes), "snr_orthogonalise_ws_bytes")
@@ -800,25 +823,28 @@ def muon_step_(params, grads, momentum_buffers, lr, momentum=0.95, nesterov=True
     args = _orth_args("muon_step_", steps, coefficients, eps, precision)
     if scale not in _MUON_SCALE:
         raise ValueError(f"muon_step_: scale must be one of {sorted(_MUON_SCALE)}, got {scale!r}")
-    (params, grads, bufs), dev = _flat_list("muon_step_", params, grads, momentum_buffers)
-    if any(p.dim() < 2 for p in params):
-        raise ValueError(f"muon_step_: expected matrices [..., m, n], got {[tuple(p.shape) for p in params if p.dim() < 2][0]}")
-    live = [i for i, p in enumerate(params) if p.numel()]
-    if not live:
+    rows, dev = _rows("muon_step_", (params, grads, momentum_buffers), 1)
+    for p, _, _ in rows:
+        if p.dim() < 2:
+            raise ValueError(f"muon_step_: expected matrices [..., m, n], got {tuple(p.shape)}")
+    rows = [r for r in rows if r[0].numel()]
+    if not rows:
         return
-    _written("muon_step_", params + bufs)
-    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
-    _no_overlap("muon_step_", grads, params + bufs)
     lib = _lib.load()
-    items = (_lib.MuonItem * len(live))(*[(params[i].data_ptr(), grads[i].data_ptr(), bufs[i].data_ptr(),
-                                           params[i].numel() // (params[i].shape[-2] * params[i].shape[-1]), params[i].shape[-2],
-                                           params[i].shape[-1]) for i in live])
+    values = []
+    for p, g, m in rows:
+        shape = p.shape
+        a, b = shape[-2], shape[-1]
+        values += (p.data_ptr(), g.data_ptr(), m.data_ptr(), 1 if len(shape) == 2 else p.numel() // (a * b), a, b)
+    items = _items(_lib.MuonItem, values)
     n_steps, a, b, c, eps, prec = args
-    with torch.cuda.device(dev):
-        nbytes = lib.snr_muon_ws_bytes(items, len(live), prec)
+    with _on(dev):
+        nbytes = lib.snr_muon_ws_bytes(items, len(rows), prec)
         if nbytes <= 0:
             check(int(nbytes), "snr_muon_ws_bytes")
-        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-        _orth_check(lib.snr_muon_step_multi(items, len(live), float(lr), float(momentum), int(bool(nesterov)), float(weight_decay),
-                                            _MUON_SCALE[scale], n_steps, a, b, c, eps, float(grad_scale), prec, ptr(state), ptr(ws),
-                                            stream()), "muon_step_", "snr_muon_step_multi")
+        ws = torch.empty(nbytes, device=rows[0][0].device, dtype=torch.uint8)
+        st = lib.snr_muon_step_multi(items, len(rows), float(lr), float(momentum), int(bool(nesterov)), float(weight_decay),
+                                     _MUON_SCALE[scale], n_steps, a, b, c, eps, float(grad_scale), prec, ptr(state), ptr(ws), stream())
+    if st:
+        _no_overlap("muon_step_", rows, 1)
+        _orth_check(st, "muon_step_", "snr_muon_step_multi")
