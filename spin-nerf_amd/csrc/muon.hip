@@ -158,7 +158,33 @@ __global__ __launch_bounds__(256) void orth_reduce_kernel(OrthArgs a, OrthArgs* 
     const int64_t base = mat * io.xb;
     const int b = io.mom ? 4 : type_bytes(a.dtype);
     const bool wide = on_grid(io.x, base * b, 0, 4 * b) && (!io.mom || on_grid(io.mom, base * 4, 0, 16));
-    for (int64_t e = e0 + 4 * threadIdx.x; e < e1; e += 1024) {
+    int64_t e = e0 + 4 * threadIdx.x;
+    constexpr int AHEAD = 4;                    // pieces a thread has in flight: one at a time is a memory latency each
+    if (wide)
+      for (; e + 1024 * (AHEAD - 1) + 4 <= e1; e += 1024 * AHEAD) {
+        f32x4 g[AHEAD], mo[AHEAD];
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) {
+          g[q] = orth_load4(io.x, base + e + 1024 * q, io.mom ? SNR_F32 : a.dtype, true);
+          if (io.mom) mo[q] = *(const f32x4*)(io.mom + base + e + 1024 * q);
+        }
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) {
+          f32x4 u = g[q];
+          if (io.mom) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float gs = g[q][i] * a.gscale;
+              mo[q][i] = mo[q][i] * a.mu + gs;
+              u[i] = a.nesterov ? gs + a.mu * mo[q][i] : mo[q][i];
+            }
+            *(f32x4*)(io.mom + base + e + 1024 * q) = mo[q];
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum += (double)u[i] * (double)u[i];
+        }
+      }
+    for (; e < e1; e += 1024) {
       f32x4 u = {0.f, 0.f, 0.f, 0.f};
       const bool whole = e + 4 <= e1;
       if (io.mom) {
@@ -694,10 +720,23 @@ __global__ __launch_bounds__(256) void orth_small_kernel(OrthArgs a, OrthOut o, 
     u.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(q + 4 * ld));
     return u.v;
   };
-  auto mul = [&](f32x16& hi, f32x16& lo, f16x8 xh, f16x8 xl, f16x8 wh, f16x8 wl) {
-    hi = __builtin_amdgcn_mfma_f32_32x32x16_f16(xh, wh, hi, 0, 0, 0);
-    lo = __builtin_amdgcn_mfma_f32_32x32x16_f16(xh, wl, lo, 0, 0, 0);
-    lo = __builtin_amdgcn_mfma_f32_32x32x16_f16(xl, wh, lo, 0, 0, 0);
+  // 64 of K: all fragments first, then the products of hi and lo planes into sums of their own (NB 7 has no registers left for a
+  // third), so that neither LDS's latency nor the matrix pipe's is waited out more than once
+  auto mul = [&](f32x16& hi, f32x16& lo, auto x, auto y) {
+    f16x8 f[4][4];
+    f32x16 other = {};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) { f[k][0] = x(0, k); f[k][1] = x(1, k); f[k][2] = y(0, k); f[k][3] = y(1, k); }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      hi = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[k][0], f[k][2], hi, 0, 0, 0);
+      lo = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[k][0], f[k][3], lo, 0, 0, 0);
+      f32x16& third = NB < 7 ? other : lo;
+      third = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[k][1], f[k][2], third, 0, 0, 0);
+    }
+    if constexpr (NB < 7) lo += other;
+    __builtin_amdgcn_sched_barrier(0);
   };
   auto put = [&](_Float16* h, _Float16* l, int ld, int i0, int j, const float (&w)[16]) {
 #pragma unroll
@@ -713,15 +752,15 @@ __global__ __launch_bounds__(256) void orth_small_kernel(OrthArgs a, OrthOut o, 
     __syncthreads();
     f32x16 hi = {}, lo = {};
 #pragma unroll
-    for (int k = 0; k < 4 * NB; ++k) mul(hi, lo, rows(yh, LD, ai, k), rows(yl, LD, ai, k), rows(yh, LD, aj, k), rows(yl, LD, aj, k));
+    for (int q = 0; q < NB; ++q)
+      mul(hi, lo, [&](int l, int k) { return rows(l ? yl : yh, LD, ai, 4 * q + k); }, [&](int l, int k) { return rows(l ? yl : yh, LD, aj, 4 * q + k); });
     float w[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) w[e] = (hi[e] + lo[e] * (1.f / kLo)) * (kAs / (kYs * kYs));
     put(ah, al, LA, ai + li, aj + lj, w);
     __syncthreads();
     hi = f32x16{}; lo = f32x16{};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) mul(hi, lo, rows(ah, LA, ai, k), rows(al, LA, ai, k), rows(ah, LA, aj, k), rows(al, LA, aj, k));
+    mul(hi, lo, [&](int l, int k) { return rows(l ? al : ah, LA, ai, k); }, [&](int l, int k) { return rows(l ? al : ah, LA, aj, k); });
 #pragma unroll
     for (int e = 0; e < 16; ++e) w[e] = cb * w[e] + cc * ((hi[e] + lo[e] * (1.f / kLo)) * (1.f / kAs));
     put(bh, bl, LA, ai + li, aj + lj, w);
@@ -730,8 +769,7 @@ __global__ __launch_bounds__(256) void orth_small_kernel(OrthArgs a, OrthOut o, 
     for (int b = 0; b < NB; ++b) {
       const int i = 32 * ((wave + 4 * b) & 1), j = 32 * ((wave + 4 * b) >> 1);
       hi = f32x16{}; lo = f32x16{};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) mul(hi, lo, rows(bh, LA, i, k), rows(bl, LA, i, k), cols(yh, LD, k, j), cols(yl, LD, k, j));
+      mul(hi, lo, [&](int l, int k) { return rows(l ? bl : bh, LA, i, k); }, [&](int l, int k) { return cols(l ? yl : yh, LD, k, j); });
 #pragma unroll
       for (int e = 0; e < 16; ++e) v[b][e] = ca * v[b][e] + (hi[e] + lo[e] * (1.f / kLo)) * (1.f / kAs);
     }
@@ -803,10 +841,10 @@ static int kind_of(int precision, int64_t m, int64_t n) {
 }
 
 using S64 = TileCfg<64, 2, 2, true, 2, 64>;
-using S128 = TileCfg<128, 2, 2, true, 2, 64>;
+using S128 = TileCfg<128, 4, 4, true, 2, 64>;
 using H64 = TileCfg<64, 2, 2, false, 3, 64>;
-using H128 = TileCfg<128, 2, 2, false, 2, 64>;
-using H192 = TileCfg<192, 2, 2, false, 3, 64>;
+using H128 = TileCfg<128, 4, 2, false, 4, 64>;
+using H192 = TileCfg<192, 6, 2, false, 3, 64>;
 using H256 = TileCfg<256, 2, 4, false, 2, 64>;
 template <int PHASE> struct Largest { using Cfg = H192; };
 template <> struct Largest<kApply> { using Cfg = H256; };
