@@ -672,38 +672,62 @@ __global__ __launch_bounds__(C::NT) void orth_product_kernel(OrthHead h, OrthOut
 constexpr int kSmallSide = 64, kSmallLong = 448;     // 448: Y's planes, A's and B's fill LDS
 template <int NB>
 __global__ __launch_bounds__(256) void orth_small_kernel(OrthArgs a, OrthOut o, float ca, float cb, float cc, int steps) {
-  constexpr int LD = 64 * NB + 8, LA = 64 + 8;       // rows in fp16: 16 B off a multiple of 128, so that 16 rows at one k spread over the banks
-  __shared__ __attribute__((aligned(16))) _Float16 yh[64 * LD], yl[64 * LD], ah[64 * LA], al[64 * LA], bh[64 * LA], bl[64 * LA];
+  constexpr int LD = 64 + 8;                         // rows in fp16: 16 B off a multiple of 128, so that 16 rows at one k spread over the banks
+  constexpr bool ROOM = NB < 7;                      // ... for B beside A
+  __shared__ __attribute__((aligned(16))) _Float16 yh[64 * NB * LD], yl[64 * NB * LD], ah[64 * LD], al[64 * LD], own[2][ROOM ? 64 * LD : 8];
+  _Float16 *bh = ROOM ? own[0] : ah, *bl = ROOM ? own[1] : al;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int s = find_item(a.sym0, blockIdx.x);
   const OrthIo& io = a.io[s];
   const int64_t mat = blockIdx.x - a.sym0[s];
   const bool tall = io.m > io.n;
-  const int r = tall ? io.n : io.m, c = tall ? io.m : io.n;
+  int r = tall ? io.n : io.m, c = tall ? io.m : io.n;
   const int lj = lane & 31, li = 4 * (lane >> 5);
+  // what lies outside the matrix is read at its last row and column, so that no load waits for a branch
   float v[NB][16];
-  double sum = 0.0;
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
+  int64_t at[16];
+  const int64_t in_i = tall ? 1 : io.xr, in_j = tall ? io.xr : 1;
+  auto where = [&](int b, int64_t base, int64_t pi, int64_t pj) {
+    __builtin_amdgcn_sched_barrier(0);               // one block's addresses at a time: seven would not fit the registers
     const int i0 = 32 * ((wave + 4 * b) & 1) + li, j = 32 * ((wave + 4 * b) >> 1) + lj;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int i = i0 + 8 * (e >> 2) + (e & 3);
-      float u = 0.f;
-      if (i < r && j < c) {
-        const int64_t at = mat * io.xb + (tall ? j * io.xr + i : i * io.xr + j);
-        if (io.mom) {
-          const float g = ((const float*)io.x)[at] * a.gscale, mo = io.mom[at] * a.mu + g;
-          io.mom[at] = mo;
-          u = a.nesterov ? g + a.mu * mo : mo;
-        } else {
-          u = orth_load(io.x, at, a.dtype);
-        }
-      }
-      v[b][e] = u;
-      sum += (double)u * (double)u;
+    for (int e = 0; e < 16; ++e) at[e] = base + min(i0 + 8 * (e >> 2) + (e & 3), r - 1) * pi + min(j, c - 1) * pj;
+  };
+  auto inside = [&](int b, int e) { return 32 * ((wave + 4 * b) & 1) + li + 8 * (e >> 2) + (e & 3) < r && 32 * ((wave + 4 * b) >> 1) + lj < c; };
+  auto fetch = [&](auto* x) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      where(b, mat * io.xb, in_i, in_j);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[b][e] = (float)x[at[e]];
     }
-  }
+  };
+  if (a.dtype == SNR_F32) fetch((const float*)io.x);
+  else if (a.dtype == SNR_F16) fetch((const _Float16*)io.x);
+  else fetch((const __bf16*)io.x);
+  if (io.mom)
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      where(b, mat * io.xb, in_i, in_j);
+      float mo[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mo[e] = io.mom[at[e]];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float g = v[b][e] * a.gscale;
+        mo[e] = mo[e] * a.mu + g;
+        v[b][e] = a.nesterov ? g + a.mu * mo[e] : mo[e];
+        if (inside(b, e)) io.mom[at[e]] = mo[e];
+      }
+    }
+  double sum = 0.0;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      if (!inside(b, e)) v[b][e] = 0.f;
+      sum += (double)v[b][e] * (double)v[b][e];
+    }
   const double norm = sqrt(block_sum(sum));
   const double scale = (double)kYs / (norm < (double)a.eps ? (double)a.eps : norm);   // (a NaN stays one)
 #pragma unroll
@@ -712,12 +736,12 @@ __global__ __launch_bounds__(256) void orth_small_kernel(OrthArgs a, OrthOut o, 
     for (int e = 0; e < 16; ++e) v[b][e] = (float)((double)v[b][e] * scale);
 
   // the operand fragments of one matrix instruction: 32 rows of a plane at 16 k, and 32 columns at 16 rows
-  auto rows = [&](const _Float16* p, int ld, int row, int k) { return *(const f16x8*)(p + (row + lj) * ld + 16 * k + 8 * (lane >> 5)); };
-  auto cols = [&](const _Float16* p, int ld, int k, int col) {
-    const _Float16* q = p + (16 * k + 8 * (lane >> 5) + ((lane & 15) >> 2)) * ld + col + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
+  auto rows = [&](const _Float16* p, int row, int k) { return *(const f16x8*)(p + (row + lj) * LD + 16 * k + 8 * (lane >> 5)); };
+  auto cols = [&](const _Float16* p, int k, int col) {
+    const _Float16* q = p + (16 * k + 8 * (lane >> 5) + ((lane & 15) >> 2)) * LD + col + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
     union { s16x4 q[2]; f16x8 v; } u;
     u.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)q);
-    u.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(q + 4 * ld));
+    u.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(q + 4 * LD));
     return u.v;
   };
   // 64 of K: all fragments first, then the products of hi and lo planes into sums of their own (NB 7 has no registers left for a
@@ -738,57 +762,68 @@ __global__ __launch_bounds__(256) void orth_small_kernel(OrthArgs a, OrthOut o, 
     if constexpr (NB < 7) lo += other;
     __builtin_amdgcn_sched_barrier(0);
   };
-  auto put = [&](_Float16* h, _Float16* l, int ld, int i0, int j, const float (&w)[16]) {
+  // a block's transpose: what a lane holds in a row then, four at a time, is a wide write.  Y lies transposed; A and B are symmetric.
+  auto put = [&](_Float16* h, _Float16* l, int i0, int j, const float (&w)[16]) {
+    typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int at = (i0 + 8 * (e >> 2) + (e & 3)) * ld + j;
-      orth_split(w[e], h[at], l[at]);
+    for (int e = 0; e < 16; e += 4) {
+      f16x4 x, y;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) { _Float16 a1, b1; orth_split(w[e + q], a1, b1); x[q] = a1; y[q] = b1; }
+      *(f16x4*)(h + j * LD + i0 + 2 * e) = x;
+      *(f16x4*)(l + j * LD + i0 + 2 * e) = y;
     }
   };
   const int ai = 32 * (wave >> 1), aj = 32 * (wave & 1);     // this wave's block of A and B
   for (int step = 0;; ++step) {
 #pragma unroll
-    for (int b = 0; b < NB; ++b) put(yh, yl, LD, 32 * ((wave + 4 * b) & 1) + li, 32 * ((wave + 4 * b) >> 1) + lj, v[b]);
+    for (int b = 0; b < NB; ++b) put(yh, yl, 32 * ((wave + 4 * b) & 1) + li, 32 * ((wave + 4 * b) >> 1) + lj, v[b]);
     __syncthreads();
     f32x16 hi = {}, lo = {};
 #pragma unroll
     for (int q = 0; q < NB; ++q)
-      mul(hi, lo, [&](int l, int k) { return rows(l ? yl : yh, LD, ai, 4 * q + k); }, [&](int l, int k) { return rows(l ? yl : yh, LD, aj, 4 * q + k); });
+      mul(hi, lo, [&](int l, int k) { return cols(l ? yl : yh, 4 * q + k, ai); }, [&](int l, int k) { return cols(l ? yl : yh, 4 * q + k, aj); });
     float w[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) w[e] = (hi[e] + lo[e] * (1.f / kLo)) * (kAs / (kYs * kYs));
-    put(ah, al, LA, ai + li, aj + lj, w);
+    put(ah, al, ai + li, aj + lj, w);
     __syncthreads();
     hi = f32x16{}; lo = f32x16{};
-    mul(hi, lo, [&](int l, int k) { return rows(l ? al : ah, LA, ai, k); }, [&](int l, int k) { return rows(l ? al : ah, LA, aj, k); });
+    mul(hi, lo, [&](int l, int k) { return rows(l ? al : ah, ai, k); }, [&](int l, int k) { return rows(l ? al : ah, aj, k); });
 #pragma unroll
     for (int e = 0; e < 16; ++e) w[e] = cb * w[e] + cc * ((hi[e] + lo[e] * (1.f / kLo)) * (1.f / kAs));
-    put(bh, bl, LA, ai + li, aj + lj, w);
+    if (!ROOM) __syncthreads();
+    put(bh, bl, ai + li, aj + lj, w);
     __syncthreads();
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       const int i = 32 * ((wave + 4 * b) & 1), j = 32 * ((wave + 4 * b) >> 1);
       hi = f32x16{}; lo = f32x16{};
-      mul(hi, lo, [&](int l, int k) { return rows(l ? bl : bh, LA, i, k); }, [&](int l, int k) { return cols(l ? yl : yh, LD, k, j); });
+      mul(hi, lo, [&](int l, int k) { return rows(l ? bl : bh, i, k); }, [&](int l, int k) { return rows(l ? yl : yh, j, k); });
 #pragma unroll
       for (int e = 0; e < 16; ++e) v[b][e] = ca * v[b][e] + (hi[e] + lo[e] * (1.f / kLo)) * (1.f / kAs);
     }
     if (step + 1 == steps) break;
     __syncthreads();
   }
+  asm volatile("" : "+s"(r), "+s"(c));                  // the tests of what lies inside are made anew: kept, they would take 2 x 16 NB registers
   float lr_q, keep;
   muon_rate(o, io, lr_q, keep);
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    const int i0 = 32 * ((wave + 4 * b) & 1) + li, j = 32 * ((wave + 4 * b) >> 1) + lj;
+    where(b, mat * io.ob, tall ? 1 : io.orow, tall ? io.orow : 1);
+    if (o.muon) {
+      float* p = (float*)io.out;
+      float x[16];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int i = i0 + 8 * (e >> 2) + (e & 3);
-      if (i >= r || j >= c) continue;
-      const int64_t at = mat * io.ob + (tall ? j * io.orow + i : i * io.orow + j);
-      const float x = v[b][e] * (1.f / kYs);
-      if (o.muon) { float* p = (float*)io.out + at; *p = *p * keep - lr_q * x; }
-      else orth_store(io.out, at, o.dtype, x);
+      for (int e = 0; e < 16; ++e) x[e] = p[at[e]];
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (inside(b, e)) p[at[e]] = x[e] * keep - lr_q * (v[b][e] * (1.f / kYs));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (inside(b, e)) orth_store(io.out, at[e], o.dtype, v[b][e] * (1.f / kYs));
     }
   }
 }
