@@ -760,9 +760,10 @@ def orthogonalise(x, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, precision=No
         X = x / max(|x|_F, eps);   steps times:  A = X X^T,  X <- a X + (b A + c A A) X        (a, b, c) = coefficients
 
     ``precision``: "fp32" = every product at fp32's accuracy, "fp16" = products of fp16 roundings (2^-11) with fp32 sums, a third of
-    the matrix work (where the shorter side is above 64; below, it is "fp32"); default "fp16" for bf16 tensors (their own roundings are coarser) and "fp32" for the others.  A zero matrix
-    gives zeros, one with a NaN or an infinity NaN throughout.  ``out`` (contiguous, may be x): where the result goes.  Not
-    differentiable: an x that requires grad is refused unless grad mode is off."""
+    the matrix work (where the shorter side is above 64; below, it is "fp32"); default "fp16" for bf16 tensors (their own roundings
+    are coarser) and "fp32" for the others.  A zero matrix gives zeros, one with a NaN or an infinity NaN throughout.  Any strides;
+    sides and stack of at most 65536.  ``out`` (contiguous, may be x): where the result goes.  Not differentiable: an x that requires
+    grad is refused unless grad mode is off."""
     if not isinstance(x, torch.Tensor) or x.dim() < 2:
         raise ValueError(f"orthogonalise: expected a tensor [..., m, n], got {tuple(x.shape) if isinstance(x, torch.Tensor) else type(x).__name__}")
     if x.dtype not in _ORTH_TYPES:
