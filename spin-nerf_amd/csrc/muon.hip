@@ -141,7 +141,8 @@ __device__ __forceinline__ double block_sum(double v) {
 }
 
 // ---- 1. momentum (in place) and the partial sums of squares of the update, in 64 bits and in a fixed order ------------------
-// A pass over the input, bound by memory: 16 B a lane where its place allows.
+// A pass over the input, bound by memory: 16 B a lane where its place allows, four of them in flight.  With the split (a pass over the
+// update, twice its bytes written): 57 us for 12.6 M parameters, gradients and momentum, 300 MB.
 __global__ __launch_bounds__(256) void orth_reduce_kernel(OrthArgs a, OrthArgs* copy) {
   if (blockIdx.x == 0) {
     static_assert(sizeof(OrthArgs) % 8 == 0, "copied as words");
@@ -298,6 +299,12 @@ __global__ __launch_bounds__(256) void orth_split_kernel(const OrthArgs* __restr
 // 16 lanes read at one k fall on different banks; Apply's Q slice has rows of T columns, read transposed (ds_read_b64_tr_b16: four k of
 // a column to a lane).  The planes are padded to 64 only: a tile that hangs over reads the last row or column again and drops what
 // comes of it.
+//
+// What bounds them.  A launch costs some 5 us however little it has to do (2 x 128 x 283: 6.5 us a product), plus a tile's first
+// slices and its epilogue; then a compute unit takes in about 88 B / ns by DMA (128-wide tiles: 32 KB and 0.37 us a slice), which is
+// what larger tiles are for, and what the products themselves reach with the whole chip on random data is 0.86 PF (4096^2, 192 and
+// 256 wide; a large library product: 1.33 PF, and zeros instead of data run 1.5 x faster here: power).  Halving the fragments'
+// reads from LDS changes nothing, nor does the order of the tiles.
 enum { kGram = 0, kPoly = 1, kApply = 2 };   // template PHASE; LAST: the result instead of planes
 
 template <int T_, int WI_, int WJ_, bool SPLIT_, int STAGES_, int BK_> struct TileCfg {
@@ -526,7 +533,7 @@ __global__ __launch_bounds__(C::NT) void orth_product_kernel(OrthHead h, OrthOut
   constexpr bool EARLY = C::TI * C::TJ == 1 && PHASE != kGram;
   const int64_t ld_out = PHASE == kApply ? G.cp : G.rp;
   Half16 eh = {}, el = {};
-  if (EARLY) {
+  if (EARLY && ti * C::T + wi < G.rp && tj * C::T + wj < ld_out) {
     const int64_t y = (int64_t)(ti * C::T + wi + (lane >> 1)) * ld_out + tj * C::T + wj + (lane & 1) * 16;
     eh = load16(W + (PHASE == kPoly ? P.ah : yh) + y);
     if (PHASE == kApply || C::SPLIT) el = load16(W + (PHASE == kPoly ? P.al : yl) + y);
@@ -890,10 +897,11 @@ struct OrthPlan { int ts, tf; int64_t sym, full, chunk, split, bytes; OrthArgs* 
 static int64_t sym_tiles(const OrthGeom& g, int T) { const int64_t t = (g.rp + T - 1) / T; return g.batch * (t * (t + 1) / 2); }
 static int64_t full_tiles(const OrthGeom& g, int T) { return (int64_t)g.batch * ((g.rp + T - 1) / T) * ((g.cp + T - 1) / T); }
 
-// The largest tile that still makes work for most of the chip: a larger one reads less per product, but a workgroup has a compute
-// unit to itself (128: two share one) and idle ones are worth more.  Us a product at 64 / 128 / 192 / 256, fp16: symmetric, 4096^2:
-// 132 / 113 / 95 / 120, 2048^2: 25 / 27 / 40 / 60; B Y, 4096^2: 249 / 170 / 198 / 135, 2048 x 8192: 125 / 89 / 102 / 80, 4 x 1024^2 and
-// 2 of 1024 x 4096: 55 / 47 / 62 / 55.  fp32 (no larger tile fits LDS twice), 2048^2: 53 / 54, 67 / 65; 14 x 256^2: 7 / 13.
+// The largest tile that still makes work for most of the chip: a larger one reads less per product, but 128 and above have a compute
+// unit to themselves and idle ones are worth more.  Us a product at 64 / 128 / the largest, fp16: symmetric, 4096^2: 119 / 105 / 81,
+// 2048 x 8192: 74 / 60 / 93, 4 x 1024^2: 16 / 15 / 21, 1400^2: 12 / 16 / 23, 14 x 256^2: 7 / 9 / 11; B Y, 4096^2: 230 / 172 / 143,
+// 2048 x 8192: 121 / 104 / 89, 1024 x 4096: 23 / 21 / 41, 1400^2: 17 / 20 / 49.  fp32 (no larger tile fits LDS twice): symmetric,
+// 2048^2: 53 / 44, 1400^2: 21 / 29; B Y, 2048^2: 67 / 59, 3 x 1024^2: 34 / 30, 1400^2: 27 / 32.
 template <class F> static int pick_tile(const OrthArgs& a, bool split, int largest, F tiles) {
   int64_t n[2] = {0, 0};
   for (int s = 0; s < a.n_geom; ++s) { n[0] += tiles(a.g[s], largest); n[1] += tiles(a.g[s], 128); }
