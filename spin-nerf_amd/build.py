@@ -23,13 +23,13 @@ SOURCES = [
     ("mlp_bwd.hip", ["-save-temps=obj"]),
     ("render_ops.hip", ["-ffp-contract=off"]),
     ("adam_pack.hip", ["-ffp-contract=off"]),    # Adam + weight pack in one kernel: must round like render_ops' adam_kernel
-    # no packed fp32 instructions: some of their forms have given wrong results on this card now and then
-    ("muon.hip", ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]),
+    ("muon.hip", []),
     ("hashgrid.hip", ["-munsafe-fp-atomics"]),   # table gradients: hardware global_atomic_add_f32, no CAS loops
     ("prof.cpp", ["-x", "hip"]),
     ("fused.cpp", ["-x", "hip"]),                # render_rays as one call: launch order only, no kernels
 ]
-COMMON = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value"]
+# no packed fp32 instructions: some of their forms have given wrong results on this card now and then
+COMMON = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _hipcc():
@@ -83,7 +83,7 @@ def _keep_listings(verbose):
 def build(force=False, verbose=True):
     os.makedirs(LIB_DIR, exist_ok=True)
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".h")]
-    headers.append(os.path.join(os.path.dirname(HERE), "include", "spinnerf_hip.h"))
+    headers += [os.path.join(os.path.dirname(HERE), "include", "spinnerf_hip.h"), os.path.abspath(__file__)]   # (the flags are here)
     objs = []
     procs = []
     for src, extra in SOURCES:
