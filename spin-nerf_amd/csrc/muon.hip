@@ -130,14 +130,17 @@ __device__ __forceinline__ bool on_grid(const void* p, int64_t a, int64_t b, int
 }
 __device__ __forceinline__ int type_bytes(int dtype) { return dtype == SNR_F32 ? 4 : 2; }
 
-// sum over the workgroup's 256 threads, in a fixed order; everyone gets it
-__device__ __forceinline__ double block_sum(double v) {
-  __shared__ double part[4];
+// sum over the workgroup's W waves, in a fixed order; everyone gets it
+template <int W = 4> __device__ __forceinline__ double block_sum(double v) {
+  __shared__ double part[W];
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
   __syncthreads();
-  return (part[0] + part[1]) + (part[2] + part[3]);
+  double sum = 0.0;
+#pragma unroll
+  for (int w = 0; w < W; w += 4) sum += (part[w] + part[w + 1]) + (part[w + 2] + part[w + 3]);
+  return sum;
 }
 
 // ---- 1. momentum (in place) and the partial sums of squares of the update, in 64 bits and in a fixed order ------------------
@@ -672,17 +675,19 @@ __global__ __launch_bounds__(C::NT) void orth_product_kernel(OrthHead h, OrthOut
 }
 
 // ---- 4. small matrices: everything in one workgroup ----------------------------------------------------------------------------------
-// Where the shorter side is 64 or less and the longer one fits, a workgroup keeps a matrix from its input to its result: 17 launches
-// of a microsecond's work each become one.  Y stays in registers in 32 bits, as 32 x 32 blocks in the layout the matrix instructions
-// give them back in (NB a wave; a wave's block never moves); LDS holds the hi and lo planes that all four waves multiply from.  Always
-// the split products.  Bound by latency: four barriers and 3 (NB + 2) dependent rounds of LDS reads and products a step.
-constexpr int kSmallSide = 64, kSmallLong = 448;     // 448: Y's planes, A's and B's fill LDS
-template <int NB>
-__global__ __launch_bounds__(256) void orth_small_kernel(OrthArgs a, OrthOut o, float ca, float cb, float cc, int steps) {
-  constexpr int LD = 64 + 8;                         // rows in fp16: 16 B off a multiple of 128, so that 16 rows at one k spread over the banks
-  constexpr bool ROOM = NB < 7;                      // ... for B beside A
-  __shared__ __attribute__((aligned(16))) _Float16 yh[64 * NB * LD], yl[64 * NB * LD], ah[64 * LD], al[64 * LD], own[2][ROOM ? 64 * LD : 8];
-  _Float16 *bh = ROOM ? own[0] : ah, *bl = ROOM ? own[1] : al;
+// Where a matrix fits, a workgroup keeps it from its input to its result: 17 launches of a microsecond's work each become one.  Y stays in
+// registers in 32 bits, as 32 x 32 blocks in the layout the matrix instructions give them back in (NB a wave; a wave's block never
+// moves); LDS holds the planes that all waves multiply from: 32 RB rows, 64 NB columns, hi and lo (SPLIT) or hi alone.  What fits
+// 160 KB beside A and B: 64 x 448 and 128 x 128 split, 128 x 320 else.  Bound by the latency of a few rounds of LDS reads and products
+// between four barriers a step, then by LDS.  Us a call, here / in tiles: 2 x 128 x 283 fp16 47 / 82, 2 x 128 x 128 fp16 29 / 70,
+// fp32 57 / 84; 1024 x 128 x 128 fp16 120 / 538, fp32 242 / 708; 64 x 64: 17 (what calling it takes), 64 x 448: 52.
+template <int RB, int NB, bool SPLIT>
+__global__ __launch_bounds__(128 * RB) void orth_small_kernel(OrthArgs a, OrthOut o, float ca, float cb, float cc, int steps) {
+  constexpr int R = 32 * RB, LD = R + (RB == 2 ? 8 : 16);             // rows in fp16: off a multiple of 128 B, so that rows at one k spread over the banks
+  constexpr bool ROOM = (64 * NB + 2 * R) * LD * (SPLIT ? 4 : 2) <= 160 * 1024 - 128;   // ... for B beside A
+  __shared__ __attribute__((aligned(16))) _Float16 yh[64 * NB * LD], yl[SPLIT ? 64 * NB * LD : 8], ah[R * LD], al[SPLIT ? R * LD : 8];
+  __shared__ __attribute__((aligned(16))) _Float16 own_h[ROOM ? R * LD : 8], own_l[ROOM && SPLIT ? R * LD : 8];
+  _Float16 *bh = ROOM ? own_h : ah, *bl = ROOM ? own_l : al;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int s = find_item(a.sym0, blockIdx.x);
   const OrthIo& io = a.io[s];
@@ -690,17 +695,20 @@ __global__ __launch_bounds__(256) void orth_small_kernel(OrthArgs a, OrthOut o, 
   const bool tall = io.m > io.n;
   int r = tall ? io.n : io.m, c = tall ? io.m : io.n;
   const int lj = lane & 31, li = 4 * (lane >> 5);
+  const int y0 = 32 * (wave % RB), x0 = 32 * (wave / RB);     // this wave's blocks of Y: at y0, x0 + 64 b
   // what lies outside the matrix is read at its last row and column, so that no load waits for a branch
   float v[NB][16];
   int64_t at[16];
   const int64_t in_i = tall ? 1 : io.xr, in_j = tall ? io.xr : 1;
   auto where = [&](int b, int64_t base, int64_t pi, int64_t pj) {
     __builtin_amdgcn_sched_barrier(0);               // one block's addresses at a time: seven would not fit the registers
-    const int i0 = 32 * ((wave + 4 * b) & 1) + li, j = 32 * ((wave + 4 * b) >> 1) + lj;
+    const int i0 = y0 + li, j = x0 + 64 * b + lj;
 #pragma unroll
     for (int e = 0; e < 16; ++e) at[e] = base + min(i0 + 8 * (e >> 2) + (e & 3), r - 1) * pi + min(j, c - 1) * pj;
   };
-  auto inside = [&](int b, int e) { return 32 * ((wave + 4 * b) & 1) + li + 8 * (e >> 2) + (e & 3) < r && 32 * ((wave + 4 * b) >> 1) + lj < c; };
+  auto inside = [&](int b, int e) { return y0 + li + 8 * (e >> 2) + (e & 3) < r && x0 + 64 * b + lj < c; };
+  // addresses and the tests of what lies inside are made anew: kept from one loop to the next, they would not fit the registers
+  auto again = [&] { asm volatile("" : "+s"(r), "+s"(c)); };
   auto fetch = [&](auto* x) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -709,16 +717,13 @@ __global__ __launch_bounds__(256) void orth_small_kernel(OrthArgs a, OrthOut o, 
       for (int e = 0; e < 16; ++e) v[b][e] = (float)x[at[e]];
     }
   };
-  if (a.dtype == SNR_F32) fetch((const float*)io.x);
-  else if (a.dtype == SNR_F16) fetch((const _Float16*)io.x);
-  else fetch((const __bf16*)io.x);
-  if (io.mom)
+  if (io.mom) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       where(b, mat * io.xb, in_i, in_j);
       float mo[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) mo[e] = io.mom[at[e]];
+      for (int e = 0; e < 16; ++e) { v[b][e] = ((const float*)io.x)[at[e]]; mo[e] = io.mom[at[e]]; }
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const float g = v[b][e] * a.gscale;
@@ -727,6 +732,14 @@ __global__ __launch_bounds__(256) void orth_small_kernel(OrthArgs a, OrthOut o, 
         if (inside(b, e)) io.mom[at[e]] = mo[e];
       }
     }
+  } else if (a.dtype == SNR_F32) {
+    fetch((const float*)io.x);
+  } else if (a.dtype == SNR_F16) {
+    fetch((const _Float16*)io.x);
+  } else {
+    fetch((const __bf16*)io.x);
+  }
+  again();
   double sum = 0.0;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
@@ -735,7 +748,7 @@ __global__ __launch_bounds__(256) void orth_small_kernel(OrthArgs a, OrthOut o, 
       if (!inside(b, e)) v[b][e] = 0.f;
       sum += (double)v[b][e] * (double)v[b][e];
     }
-  const double norm = sqrt(block_sum(sum));
+  const double norm = sqrt(block_sum<2 * RB>(sum));
   const double scale = (double)kYs / (norm < (double)a.eps ? (double)a.eps : norm);   // (a NaN stays one)
 #pragma unroll
   for (int b = 0; b < NB; ++b)
@@ -751,24 +764,32 @@ __global__ __launch_bounds__(256) void orth_small_kernel(OrthArgs a, OrthOut o, 
     u.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(q + 4 * LD));
     return u.v;
   };
-  // 64 of K: all fragments first, then the products of hi and lo planes into sums of their own (NB 7 has no registers left for a
-  // third), so that neither LDS's latency nor the matrix pipe's is waited out more than once
-  auto mul = [&](f32x16& hi, f32x16& lo, auto x, auto y) {
-    f16x8 f[4][4];
-    f32x16 other = {};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) { f[k][0] = x(0, k); f[k][1] = x(1, k); f[k][2] = y(0, k); f[k][3] = y(1, k); }
-    __builtin_amdgcn_sched_barrier(0);
+  // 64 of K of an operand: all fragments ahead of the products, so that LDS's latency is not waited out more than once
+  struct Frag64 { f16x8 h[4], l[SPLIT ? 4 : 1]; };
+  auto take = [&](Frag64& f, const _Float16* h, const _Float16* l, auto get) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      hi = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[k][0], f[k][2], hi, 0, 0, 0);
-      lo = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[k][0], f[k][3], lo, 0, 0, 0);
-      f32x16& third = NB < 7 ? other : lo;
-      third = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[k][1], f[k][2], third, 0, 0, 0);
+      f.h[k] = get(h, k);
+      if constexpr (SPLIT) f.l[k] = get(l, k);
     }
-    if constexpr (NB < 7) lo += other;
-    __builtin_amdgcn_sched_barrier(0);
   };
+  // ... and the products, of hi and lo planes into sums of their own (a third where there are registers for it: the next one that adds to
+  // the same sum has to wait)
+  auto mul = [&](f32x16& hi, f32x16& lo, const Frag64& x, const Frag64& y) {
+    constexpr bool THIRD = SPLIT && RB == 2 && NB < 7;
+    f32x16 other = {};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      hi = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.h[k], y.h[k], hi, 0, 0, 0);
+      if constexpr (SPLIT) {
+        lo = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.h[k], y.l[k], lo, 0, 0, 0);
+        f32x16& third = THIRD ? other : lo;
+        third = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.l[k], y.h[k], third, 0, 0, 0);
+      }
+    }
+    if constexpr (THIRD) lo += other;
+  };
+  auto both = [&](const f32x16& hi, const f32x16& lo, int e) { return SPLIT ? hi[e] + lo[e] * (1.f / kLo) : hi[e]; };
   // a block's transpose: what a lane holds in a row then, four at a time, is a wide write.  Y lies transposed; A and B are symmetric.
   auto put = [&](_Float16* h, _Float16* l, int i0, int j, const float (&w)[16]) {
     typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
@@ -778,42 +799,75 @@ __global__ __launch_bounds__(256) void orth_small_kernel(OrthArgs a, OrthOut o, 
 #pragma unroll
       for (int q = 0; q < 4; ++q) { _Float16 a1, b1; orth_split(w[e + q], a1, b1); x[q] = a1; y[q] = b1; }
       *(f16x4*)(h + j * LD + i0 + 2 * e) = x;
-      *(f16x4*)(l + j * LD + i0 + 2 * e) = y;
+      if constexpr (SPLIT) *(f16x4*)(l + j * LD + i0 + 2 * e) = y;
     }
   };
-  const int ai = 32 * (wave >> 1), aj = 32 * (wave & 1);     // this wave's block of A and B
+  constexpr int AB = RB / 2;                                  // this wave's blocks of A and B: at a0 + 64 n, a1
+  const int a0 = 32 * (wave / RB), a1 = 32 * (wave % RB);
   for (int step = 0;; ++step) {
 #pragma unroll
-    for (int b = 0; b < NB; ++b) put(yh, yl, 32 * ((wave + 4 * b) & 1) + li, 32 * ((wave + 4 * b) >> 1) + lj, v[b]);
+    for (int b = 0; b < NB; ++b) put(yh, yl, y0 + li, x0 + 64 * b + lj, v[b]);
     __syncthreads();
-    f32x16 hi = {}, lo = {};
+    float w[AB][16];
+    f32x16 hi[AB] = {}, lo[AB] = {};
 #pragma unroll
-    for (int q = 0; q < NB; ++q)
-      mul(hi, lo, [&](int l, int k) { return cols(l ? yl : yh, 4 * q + k, ai); }, [&](int l, int k) { return cols(l ? yl : yh, 4 * q + k, aj); });
-    float w[16];
+    for (int q = 0; q < NB; ++q) {
+      Frag64 x[AB], y;
+      take(y, yh, yl, [&](const _Float16* p, int k) { return cols(p, 4 * q + k, a1); });
 #pragma unroll
-    for (int e = 0; e < 16; ++e) w[e] = (hi[e] + lo[e] * (1.f / kLo)) * (kAs / (kYs * kYs));
-    put(ah, al, ai + li, aj + lj, w);
+      for (int n = 0; n < AB; ++n) take(x[n], yh, yl, [&](const _Float16* p, int k) { return cols(p, 4 * q + k, a0 + 64 * n); });
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int n = 0; n < AB; ++n) mul(hi[n], lo[n], x[n], y);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int n = 0; n < AB; ++n) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) w[n][e] = both(hi[n], lo[n], e) * (kAs / (kYs * kYs));
+      put(ah, al, a0 + 64 * n + li, a1 + lj, w[n]);
+      hi[n] = f32x16{}; lo[n] = f32x16{};
+    }
     __syncthreads();
-    hi = f32x16{}; lo = f32x16{};
-    mul(hi, lo, [&](int l, int k) { return rows(l ? al : ah, ai, k); }, [&](int l, int k) { return rows(l ? al : ah, aj, k); });
 #pragma unroll
-    for (int e = 0; e < 16; ++e) w[e] = cb * w[e] + cc * ((hi[e] + lo[e] * (1.f / kLo)) * (1.f / kAs));
+    for (int q = 0; q < AB; ++q) {
+      Frag64 x[AB], y;
+      take(y, ah, al, [&](const _Float16* p, int k) { return rows(p, a1, 4 * q + k); });
+#pragma unroll
+      for (int n = 0; n < AB; ++n) take(x[n], ah, al, [&](const _Float16* p, int k) { return rows(p, a0 + 64 * n, 4 * q + k); });
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int n = 0; n < AB; ++n) mul(hi[n], lo[n], x[n], y);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     if (!ROOM) __syncthreads();
-    put(bh, bl, ai + li, aj + lj, w);
+#pragma unroll
+    for (int n = 0; n < AB; ++n) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) w[n][e] = cb * w[n][e] + cc * (both(hi[n], lo[n], e) * (1.f / kAs));
+      put(bh, bl, a0 + 64 * n + li, a1 + lj, w[n]);
+    }
     __syncthreads();
+    Frag64 x[AB];
+#pragma unroll
+    for (int q = 0; q < AB; ++q) take(x[q], bh, bl, [&](const _Float16* p, int k) { return rows(p, y0, 4 * q + k); });
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      const int i = 32 * ((wave + 4 * b) & 1), j = 32 * ((wave + 4 * b) >> 1);
-      hi = f32x16{}; lo = f32x16{};
-      mul(hi, lo, [&](int l, int k) { return rows(l ? bl : bh, i, k); }, [&](int l, int k) { return rows(l ? yl : yh, j, k); });
+      f32x16 h = {}, l = {};
+      Frag64 y[AB];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) v[b][e] = ca * v[b][e] + (hi[e] + lo[e] * (1.f / kLo)) * (1.f / kAs);
+      for (int q = 0; q < AB; ++q) take(y[q], yh, yl, [&](const _Float16* p, int k) { return rows(p, x0 + 64 * b, 4 * q + k); });
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int q = 0; q < AB; ++q) mul(h, l, x[q], y[q]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[b][e] = ca * v[b][e] + both(h, l, e) * (1.f / kAs);
     }
     if (step + 1 == steps) break;
     __syncthreads();
   }
-  asm volatile("" : "+s"(r), "+s"(c));                  // the tests of what lies inside are made anew: kept, they would take 2 x 16 NB registers
+  again();
   float lr_q, keep;
   muon_rate(o, io, lr_q, keep);
 #pragma unroll
@@ -874,12 +928,16 @@ static int stack_ok(int64_t batch, int64_t m, int64_t n) {
   if (batch < 1 || m < 1 || n < 1 || m > kMaxSide || n > kMaxSide || batch > kMaxBatch) return SNR_ERR_SHAPE;
   return SNR_OK;
 }
-// What a matrix goes through: the small kernel at NB = 1, 2, 4 or 7, the split products, or fp16 products.
-enum { kSmall1 = 0, kSmall2, kSmall4, kSmall7, kSplit, kHalf, kKinds };
+// What a matrix goes through: one workgroup (64 or 128 rows, so many columns, split or hi planes alone), the split products of tiles, or
+// fp16 products of tiles.
+enum { kSmall64, kSmall128, kSmall256, kSmall448, kMid128, kMid128h, kMid192h, kMid320h, kSplit, kHalf, kKinds };
 static int kind_of(int precision, int64_t m, int64_t n) {
   const int64_t r = m < n ? m : n, c = m < n ? n : m;
-  if (r <= kSmallSide && c <= kSmallLong) return c <= 64 ? kSmall1 : c <= 128 ? kSmall2 : c <= 256 ? kSmall4 : kSmall7;
-  return precision == SNR_ORTH_FP32 || r <= 64 ? kSplit : kHalf;
+  const bool split = precision == SNR_ORTH_FP32 || r <= 64;
+  if (r <= 64 && c <= 448) return c <= 64 ? kSmall64 : c <= 128 ? kSmall128 : c <= 256 ? kSmall256 : kSmall448;
+  if (r <= 128 && split && c <= 128) return kMid128;
+  if (r <= 128 && !split && c <= 320) return c <= 128 ? kMid128h : c <= 192 ? kMid192h : kMid320h;
+  return split ? kSplit : kHalf;
 }
 
 using S64 = TileCfg<64, 2, 2, true, 2, 64>;
@@ -988,12 +1046,16 @@ static int orth_run(OrthArgs& a, const OrthOut& o, int steps, float ca, float cb
   const bool split = kind != kHalf;
   if (kind < kSplit) {
     ProfScope ps(K_ORTH_SMALL, st);
-    const dim3 n((unsigned)p.sym), t(256);
+    const dim3 n((unsigned)p.sym);
     switch (kind) {
-      case kSmall1: orth_small_kernel<1><<<n, t, 0, st>>>(a, o, ca, cb, cc, steps); break;
-      case kSmall2: orth_small_kernel<2><<<n, t, 0, st>>>(a, o, ca, cb, cc, steps); break;
-      case kSmall4: orth_small_kernel<4><<<n, t, 0, st>>>(a, o, ca, cb, cc, steps); break;
-      default: orth_small_kernel<7><<<n, t, 0, st>>>(a, o, ca, cb, cc, steps);
+      case kSmall64: orth_small_kernel<2, 1, true><<<n, dim3(256), 0, st>>>(a, o, ca, cb, cc, steps); break;
+      case kSmall128: orth_small_kernel<2, 2, true><<<n, dim3(256), 0, st>>>(a, o, ca, cb, cc, steps); break;
+      case kSmall256: orth_small_kernel<2, 4, true><<<n, dim3(256), 0, st>>>(a, o, ca, cb, cc, steps); break;
+      case kSmall448: orth_small_kernel<2, 7, true><<<n, dim3(256), 0, st>>>(a, o, ca, cb, cc, steps); break;
+      case kMid128: orth_small_kernel<4, 2, true><<<n, dim3(512), 0, st>>>(a, o, ca, cb, cc, steps); break;
+      case kMid128h: orth_small_kernel<4, 2, false><<<n, dim3(512), 0, st>>>(a, o, ca, cb, cc, steps); break;
+      case kMid192h: orth_small_kernel<4, 3, false><<<n, dim3(512), 0, st>>>(a, o, ca, cb, cc, steps); break;
+      default: orth_small_kernel<4, 5, false><<<n, dim3(512), 0, st>>>(a, o, ca, cb, cc, steps);
     }
     return launch_status();
   }

@@ -43,6 +43,26 @@ def test_muon_with_large_tiles_and_with_many_sizes(S, shapes, precision):
         assert bool((off <= tol).all()), (float(off.max()), float(tol.min()))
 
 
+# what one workgroup keeps: 64 x 448 and 128 x 128 at fp32's accuracy, 128 x 320 with fp16 products; both sides of each edge
+@pytest.mark.parametrize("m,n", [(64, 65), (65, 65), (66, 129), (128, 128), (129, 128), (128, 192), (193, 128), (100, 319), (320, 128), (70, 321), (448, 64)])
+@pytest.mark.parametrize("precision", ["fp32", "fp16"])
+def test_sizes_around_what_one_workgroup_keeps(S, m, n, precision):
+    gen = torch.Generator().manual_seed(m + n)
+    for dtype in (torch.float32, torch.bfloat16):
+        x = gradient_like(gen, 2, m, n).to(dtype)
+        check(S.orthogonalise(x.cuda(), precision=precision), x, precision)
+    p, g, b = muon_case(gen, [(3, m, n), (n, m)])
+    dp, dg, db = ([t.cuda() for t in ts] for ts in (p, g, b))
+    S.muon_step_(dp, dg, db, 0.02, weight_decay=0.1, precision=precision)
+    for P, G, M, gp, gm in zip(p, g, b, dp, db):
+        rp, rm, step, o, norms = muon_oracle(P, G, M, 0.02, 0.95, True, 0.1, "spectral", 1.0)
+        assert float((gm.cpu().double() - rm).norm()) <= 3 * 2.0 ** -24 * float(rm.norm() + G.double().norm())
+        off, size = (gp.cpu().double() - rp).flatten(-2).norm(dim=-1), o.flatten(-2).norm(dim=-1)
+        tol = step * ((HALF * size if precision == "fp16" else bound32(norms, 5, NS[0])) + 485 * 4 * 2.0 ** -24) \
+            + 4 * 2.0 ** -24 * P.double().flatten(-2).norm(dim=-1)
+        assert bool((off <= tol).all()), (float(off.max()), float(tol.min()))
+
+
 @pytest.mark.parametrize("n", [1, 33, 64, 100, 300])
 def test_diagonal_and_mostly_empty_matrices(S, n):
     """a diagonal one keeps its zeros exactly, in either precision: no product of two different rows has a nonzero term"""
