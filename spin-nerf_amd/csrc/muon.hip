@@ -1110,9 +1110,36 @@ extern "C" int snr_orthogonalise(const void* x, int dtype, int64_t batch, int64_
   return orth_run(A, o, steps, a, b, c, kind_of(precision, rows, cols), (char*)ws, (hipStream_t)stream);
 }
 
+// Where the matrices of each kind go in a call that has several: sequences run one after the other, and one that does little takes its
+// latency all the same (us: 17 .. 55 for one workgroup a matrix, 70 .. 125 for tiles).  Those that would fit a workgroup therefore go
+// with the tiles if there are any at their precision and their own tiles are one for each compute unit at most, and those of several
+// widths go with the widest, up to one matrix for each.  Us together / apart, with 14 x 256^2: 2 x 128 x 128 fp16 90 / 120, fp32
+// 115 / 174; 64 x 128 x 128 109 / 121, 152 / 175; 64 x 64 x 448 fp32 209 / 176.  64 x 64, x 100, x 200 and x 400: 54 / 133.
+static void merge_kinds(const snr_muon_item* items, int n_items, int precision, int (&to)[kKinds]) {
+  int64_t n[kKinds] = {}, tiles[kKinds] = {};
+  for (int i = 0; i < n_items; ++i) {
+    const snr_muon_item& it = items[i];
+    const int k = kind_of(precision, it.rows, it.cols);
+    n[k] += it.batch;
+    tiles[k] += it.batch * ((it.rows + kPad - 1) / kPad) * ((it.cols + kPad - 1) / kPad);
+  }
+  for (int k = 0; k < kKinds; ++k) to[k] = k;
+  const int cus = cu_count();
+  const struct { int first, last, with; } groups[] = {{kSmall64, kSmall448, kSplit}, {kMid128, kMid128, kSplit}, {kMid128h, kMid320h, kHalf}};
+  for (const auto& g : groups) {
+    int64_t total = 0, work = 0;
+    int widest = g.first;
+    for (int k = g.first; k <= g.last; ++k) { total += n[k]; work += tiles[k]; widest = n[k] ? k : widest; }
+    const bool join = n[g.with] && work <= cus;
+    for (int k = g.first; k <= g.last; ++k) to[k] = join ? g.with : total <= cus ? widest : k;
+  }
+}
+
 // The launch sequences of a list of items: stacks of one kind share one, kOrthMax at a time; they run one after the other and share
 // the workspace.  F(OrthArgs&, kind) returns a status.
 template <class F> static int for_sequences(const snr_muon_item* items, int n_items, int precision, F f) {
+  int to[kKinds];
+  merge_kinds(items, n_items, precision, to);
   for (int kind = 0; kind < kKinds; ++kind) {
     OrthArgs A{};
     for (int i = 0; i <= n_items; ++i) {
@@ -1123,7 +1150,7 @@ template <class F> static int for_sequences(const snr_muon_item* items, int n_it
       }
       if (i == n_items) break;
       const snr_muon_item& it = items[i];
-      if (kind_of(precision, it.rows, it.cols) != kind) continue;
+      if (to[kind_of(precision, it.rows, it.cols)] != kind) continue;
       const int64_t mn = it.rows * it.cols;
       A.io[A.n_items++] = OrthIo{it.grads, it.params, it.momentum, mn, it.cols, mn, it.cols, (int)it.rows, (int)it.cols, (int)it.batch, 0, 0, 0, 0};
     }
