@@ -231,6 +231,7 @@ __global__ __launch_bounds__(kApThreads) void adam_pack_kernel(AdamPackArgs a) {
 // every workgroup has at hand, instead of a table that would have to be copied first.
 constexpr int kAdamMulti = 48;   // ranges per launch: the kernel arguments hold the table
 constexpr int kAmThreads = 256, kAmBlock = 4 * kAmThreads;   // values per workgroup
+constexpr int64_t kAmMost = (1 << 24) - 1;                   // workgroups: a launch has less than 2^32 threads
 struct AdamRange { float* p; const float* g; float* m; float* v; int64_t n; int64_t block0; };
 struct AdamMultiArgs {
   AdamRange r[kAdamMulti];
@@ -356,7 +357,7 @@ extern "C" int snr_adam_step_multi(const snr_adam_item* items, int n_items, floa
   SNR_CHECK_ARG(items, SNR_ERR_NULL);
   SNR_CHECK_ARG(n_items >= 1 && (state || step >= 1), SNR_ERR_SHAPE);
   for (int i = 0; i < n_items; ++i) {
-    SNR_CHECK_ARG(items[i].n >= 0 && items[i].n <= (int64_t)1 << 40, SNR_ERR_SHAPE);
+    SNR_CHECK_ARG(items[i].n >= 0 && items[i].n <= kAmMost * kAmBlock, SNR_ERR_SHAPE);
     SNR_CHECK_ARG(items[i].n == 0 || (items[i].params && items[i].grads && items[i].exp_avg && items[i].exp_avg_sq), SNR_ERR_NULL);
   }
   Span* spans = (Span*)malloc(sizeof(Span) * 4 * (size_t)n_items);
@@ -378,7 +379,7 @@ extern "C" int snr_adam_step_multi(const snr_adam_item* items, int n_items, floa
       const snr_adam_item& it = items[i];
       if (it.n == 0) continue;
       const int64_t nb = (it.n + kAmBlock - 1) / kAmBlock;
-      if (blocks + nb > INT32_MAX) break;       // (the next launch takes it)
+      if (blocks + nb > kAmMost) break;         // (the next launch takes it)
       a.r[a.n++] = AdamRange{it.params, it.grads, it.exp_avg, it.exp_avg_sq, it.n, blocks};
       blocks += nb;
     }

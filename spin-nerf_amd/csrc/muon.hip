@@ -924,6 +924,7 @@ static bool orth_bounded(int steps, double a, double b, double c) {
 
 static int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 static const int64_t kMaxSide = 65536, kMaxBatch = 65536;
+static const int64_t kMaxBlocks = 1 << 22;      // a launch is at most 2^32 threads, 1024 a workgroup
 static int stack_ok(int64_t batch, int64_t m, int64_t n) {
   if (batch < 1 || m < 1 || n < 1 || m > kMaxSide || n > kMaxSide || batch > kMaxBatch) return SNR_ERR_SHAPE;
   return SNR_OK;
@@ -992,7 +993,7 @@ static int orth_plan(OrthArgs& a, int kind, OrthPlan& p) {
     io.part = part; part += (int64_t)io.batch * io.nchunk;
     a.chunk0[s] = (int)p.chunk; p.chunk += (int64_t)io.batch * io.nchunk;
     a.split0[s] = (int)p.split; p.split += (int64_t)io.batch * (g.rp / kPad) * (g.cp / kPad);
-    if (p.chunk > INT32_MAX || p.split > INT32_MAX) return SNR_ERR_SHAPE;
+    if (p.chunk > kMaxBlocks || p.split > kMaxBlocks) return SNR_ERR_SHAPE;
   }
   p.ts = pick_tile(a, split, 192, sym_tiles);
   p.tf = pick_tile(a, split, 256, full_tiles);

@@ -81,3 +81,14 @@ def test_workspace_sizes(S):
     it = (L.MuonItem * 30)(*[L.MuonItem(256, 256, 256, 1, 64, 64)] * 30)
     assert lib.snr_muon_ws_bytes(it, 1, 0) > 0 and lib.snr_muon_ws_bytes(it, 30, 0) >= lib.snr_muon_ws_bytes(it, 2, 0)
     assert lib.snr_muon_ws_bytes(None, 1, 0) == -1 and lib.snr_muon_ws_bytes(it, 0, 0) == -2
+
+
+def test_launches_past_the_largest_grid_are_refused(S):
+    """a launch holds fewer than 2^32 threads: 2^22 workgroups of up to 1024, 2^24 of 256 (each with 1024 of Adam's values)"""
+    lib, L = S._lib.load(), S._lib
+    assert lib.snr_orthogonalise_ws_bytes(65536, 1, 65536, 0) == -2              # 1024 tiles a matrix
+    assert lib.snr_orthogonalise_ws_bytes(4096, 1, 65536, 0) > 0
+    it = (L.MuonItem * 2)(L.MuonItem(256, 256, 256, 4096, 1, 65536), L.MuonItem(256, 256, 256, 1, 1, 65536))
+    assert lib.snr_muon_ws_bytes(it, 1, 0) > 0 and lib.snr_muon_ws_bytes(it, 2, 0) == -2
+    ad = (L.AdamItem * 1)(L.AdamItem(256, 256, 256, 256, 1 << 34))
+    assert lib.snr_adam_step_multi(ad, 1, 1e-3, 0.9, 0.999, 1e-8, 1, 1.0, None, None) == -2
