@@ -305,8 +305,8 @@ __global__ __launch_bounds__(256) void orth_split_kernel(const OrthArgs* __restr
 //
 // What bounds them.  A launch costs some 5 us however little it has to do (2 x 128 x 283: 6.5 us a product), plus a tile's first
 // slices and its epilogue; then a compute unit takes in about 88 B / ns by DMA (128-wide tiles: 32 KB and 0.37 us a slice), which is
-// what larger tiles are for, and what the products themselves reach with the whole chip on random data is 0.86 PF (4096^2, 192 and
-// 256 wide; a large library product: 1.33 PF, and zeros instead of data run 1.5 x faster here: power).  Halving the fragments'
+// what larger tiles are for, and what the products themselves reach with the whole chip on random data is 0.92 PF (4096^2, 192 and
+// 256 wide; a large library product: 1.33 PF, and zeros instead of data run 1.3 .. 1.5 x faster here: power).  Halving the fragments'
 // reads from LDS changes nothing, nor does the order of the tiles.
 enum { kGram = 0, kPoly = 1, kApply = 2 };   // template PHASE; LAST: the result instead of planes
 
@@ -683,7 +683,7 @@ __global__ __launch_bounds__(C::NT) void orth_product_kernel(OrthHead h, OrthOut
 // fp32 57 / 84; 1024 x 128 x 128 fp16 120 / 538, fp32 242 / 708; 64 x 64: 17 (what calling it takes), 64 x 448: 52.
 template <int RB, int NB, bool SPLIT>
 __global__ __launch_bounds__(128 * RB) void orth_small_kernel(OrthArgs a, OrthOut o, float ca, float cb, float cc, int steps) {
-  constexpr int R = 32 * RB, LD = R + (RB == 2 ? 8 : 16);             // rows in fp16: off a multiple of 128 B, so that rows at one k spread over the banks
+  constexpr int R = 32 * RB, LD = R + (RB == 2 ? 8 : 16);    // rows in fp16: off a multiple of 128 B, so that rows at one k spread over the banks
   constexpr bool ROOM = (64 * NB + 2 * R) * LD * (SPLIT ? 4 : 2) <= 160 * 1024 - 128;   // ... for B beside A
   __shared__ __attribute__((aligned(16))) _Float16 yh[64 * NB * LD], yl[SPLIT ? 64 * NB * LD : 8], ah[R * LD], al[SPLIT ? R * LD : 8];
   __shared__ __attribute__((aligned(16))) _Float16 own_h[ROOM ? R * LD : 8], own_l[ROOM && SPLIT ? R * LD : 8];
