@@ -944,11 +944,14 @@ static int kind_of(int precision, int64_t m, int64_t n) {
 using S64 = TileCfg<64, 2, 2, true, 2, 64>;
 using S128 = TileCfg<128, 4, 4, true, 2, 64>;
 using H64 = TileCfg<64, 2, 2, false, 3, 64>;
-using H128 = TileCfg<128, 4, 2, false, 4, 64>;
-using H192 = TileCfg<192, 6, 2, false, 3, 64>;
-using H256 = TileCfg<256, 2, 4, false, 2, 64>;
-template <int PHASE> struct Largest { using Cfg = H192; };
-template <> struct Largest<kApply> { using Cfg = H256; };
+template <int PHASE> struct Half {                     // fp16 products: 128, and the largest
+  using T128 = TileCfg<128, 4, 2, false, 4, 64>;       // deep: mostly one round of tiles
+  using Most = TileCfg<192, 6, 2, false, 3, 64>;
+};
+template <> struct Half<kApply> {
+  using T128 = TileCfg<128, 2, 4, false, 2, 64>;       // two a compute unit, so that one writes its planes while the other multiplies
+  using Most = TileCfg<256, 2, 4, false, 2, 64>;
+};
 
 // Everything of a launch sequence that follows from its stacks' sizes; also the bytes of its workspace.
 struct OrthPlan { int ts, tf; int64_t sym, full, chunk, split, bytes; OrthArgs* args; };
@@ -956,17 +959,28 @@ struct OrthPlan { int ts, tf; int64_t sym, full, chunk, split, bytes; OrthArgs* 
 static int64_t sym_tiles(const OrthGeom& g, int T) { const int64_t t = (g.rp + T - 1) / T; return g.batch * (t * (t + 1) / 2); }
 static int64_t full_tiles(const OrthGeom& g, int T) { return (int64_t)g.batch * ((g.rp + T - 1) / T) * ((g.cp + T - 1) / T); }
 
-// The largest tile that still makes work for most of the chip: a larger one reads less per product, but 128 and above have a compute
-// unit to themselves and idle ones are worth more.  Us a product at 64 / 128 / the largest, fp16: symmetric, 4096^2: 119 / 105 / 81,
-// 2048 x 8192: 74 / 60 / 93, 4 x 1024^2: 16 / 15 / 21, 1400^2: 12 / 16 / 23, 14 x 256^2: 7 / 9 / 11; B Y, 4096^2: 230 / 172 / 143,
-// 2048 x 8192: 121 / 104 / 89, 1024 x 4096: 23 / 21 / 41, 1400^2: 17 / 20 / 49.  fp32 (no larger tile fits LDS twice): symmetric,
-// 2048^2: 53 / 44, 1400^2: 21 / 29; B Y, 2048^2: 67 / 59, 3 x 1024^2: 34 / 30, 1400^2: 27 / 32.
-template <class F> static int pick_tile(const OrthArgs& a, bool split, int largest, F tiles) {
-  int64_t n[2] = {0, 0};
-  for (int s = 0; s < a.n_geom; ++s) { n[0] += tiles(a.g[s], largest); n[1] += tiles(a.g[s], 128); }
-  const int cus = cu_count();
-  if (!split && n[0] >= cus * 3 / 4) return largest;
-  return n[1] >= cus / 2 ? 128 : 64;
+// Tiles of 64, 128 and, for fp16 products, 192 (symmetric) or 256 (B Y).  A larger one reads less per product, but 128 and above have a
+// compute unit to themselves and idle ones are worth more: 128 from half the chip on.  Us a product at 64 / 128, fp16: symmetric,
+// 2048^2 (136 tiles of 128): 24 / 22, 4 x 1024^2 (144): 16 / 15, 3 x 1024^2 (108): 12 / 14; B Y, 1024 x 4096: 23 / 21, 1400^2: 17 / 20.  fp32
+// (no larger tile fits LDS twice): symmetric, 2048^2: 53 / 44, 1400^2: 21 / 29; B Y, 2048^2: 67 / 59, 3 x 1024^2: 34 / 30.
+static int pick_tile(int64_t n128) { return n128 >= cu_count() / 2 ? 128 : 64; }
+// 128 or 192: a round of tiles (one a compute unit) takes as long as a tile's rows take to come in, the products of the whole chip as long
+// as its power allows, whichever is more; and every round after the first has an epilogue that nothing hides.  Us at 128 / 192: 4096^2
+// (528 / 253 tiles): 105 / 81, 2048^2 (136 / 66): 22 / 32, 13 x 1024^2 (468 / 273): 27 / 38, 2 x 2048 x 3000 (272 / 132): 50 / 42, 3 x 2048^2
+// (408 / 198): 40 / 38, 5 x 1500^2 (390 / 180): 32 / 30.
+static int pick_sym(int64_t n128, int64_t n192) {
+  const int64_t cus = cu_count();
+  auto cost = [&](double T, int64_t n, double slower) {
+    const double rounds = (double)((n + cus - 1) / cus);
+    return fmax(rounds * T * slower, (double)n * T * T / (99.0 * (double)cus)) * (0.9 + 0.1 * rounds);
+  };
+  return pick_tile(n128) == 128 && cost(192, n192, 1.13) < cost(128, n128, 1.0) ? 192 : pick_tile(n128);
+}
+// 128 or 256: 256 where its rounds are more than three quarters full.  Us at 128 / 256: 4096^2 (256 tiles of 256): 144 / 133, 2048 x 7000
+// (224): 82 / 77, 3500^2 (196): 120 / 106, 3 x 2048^2 (192): 73 / 77, 12 x 512 x 2048 (192): 34 / 40, 5 x 1500^2 (180): 58 / 61.
+static int pick_full(int64_t n128, int64_t n256) {
+  const int64_t cus = cu_count(), room = (n256 + cus - 1) / cus * cus;
+  return pick_tile(n128) == 128 && 4 * n256 > 3 * room ? 256 : pick_tile(n128);
 }
 
 static int orth_plan(OrthArgs& a, int kind, OrthPlan& p) {
@@ -995,8 +1009,13 @@ static int orth_plan(OrthArgs& a, int kind, OrthPlan& p) {
     a.split0[s] = (int)p.split; p.split += (int64_t)io.batch * (g.rp / kPad) * (g.cp / kPad);
     if (p.chunk > kMaxBlocks || p.split > kMaxBlocks) return SNR_ERR_SHAPE;
   }
-  p.ts = pick_tile(a, split, 192, sym_tiles);
-  p.tf = pick_tile(a, split, 256, full_tiles);
+  int64_t ns[2] = {0, 0}, nf[2] = {0, 0};
+  for (int s = 0; s < a.n_geom; ++s) {
+    ns[0] += sym_tiles(a.g[s], 128); ns[1] += sym_tiles(a.g[s], 192);
+    nf[0] += full_tiles(a.g[s], 128); nf[1] += full_tiles(a.g[s], 256);
+  }
+  p.ts = split ? pick_tile(ns[0]) : pick_sym(ns[0], ns[1]);
+  p.tf = split ? pick_tile(nf[0]) : pick_full(nf[0], nf[1]);
   for (int s = 0; s < a.n_geom; ++s) {       // (no more tiles than the split's: one holds 64 x 64 or more)
     OrthGeom& g = a.g[s];
     g.ws = off; off += (int64_t)g.batch * orth_planes(g.rp, g.cp, split).total * 2;
@@ -1032,9 +1051,9 @@ static void launch_tile(bool split, int T, const OrthHead& a, const OrthOut& o, 
   } else if (T == 64) {
     launch<PHASE, last, H64>(a, o, n, ca, cb, cc, flip, st);
   } else if (T == 128) {
-    launch<PHASE, last, H128>(a, o, n, ca, cb, cc, flip, st);
+    launch<PHASE, last, typename Half<PHASE>::T128>(a, o, n, ca, cb, cc, flip, st);
   } else {
-    launch<PHASE, last, typename Largest<PHASE>::Cfg>(a, o, n, ca, cb, cc, flip, st);
+    launch<PHASE, last, typename Half<PHASE>::Most>(a, o, n, ca, cb, cc, flip, st);
   }
 }
 
