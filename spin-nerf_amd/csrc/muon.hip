@@ -58,7 +58,7 @@ struct OrthHead {
   char* ws;
   int n;                 // 0: look them up in args
   int first[kHead];      // of the phase
-  int pad;
+  int spread;            // every XCD has its part of every geometry
   OrthGeom g[kHead];
 };
 struct OrthOut {         // the last product's epilogue
@@ -447,11 +447,11 @@ __device__ __forceinline__ void store16_out(void* p, int64_t i, int dtype, const
   }
 }
 
-// Workgroups go round the 8 XCDs, each with its own L2: number them so that an XCD has a run of neighbours, which share operand rows.
-__device__ __forceinline__ int xcd_block() {
-  const int n = gridDim.x, q = n >> 3, rem = n & 7, x = blockIdx.x & 7;
-  return x * q + (x < rem ? x : rem) + (blockIdx.x >> 3);
-}
+// Workgroups go round the 8 XCDs, each with its own L2: number n of them (a multiple of 8) so that an XCD has a run of neighbours, which
+// share operand rows.  Of the whole launch, or, where geometries differ in K, of each: an XCD with all the long ones would be the last
+// (us, fp32: 2048^2 with 2048 x 8192 3310 -> 2630, eight of 512^2 with four of 512 x 2048 434 -> 398; but 7 of 256^2 with 256 x 319 and
+// 128 x 283 125 -> 131, where a small geometry is better off in one L2).
+__device__ __forceinline__ int xcd_block(int k, int n) { return (k & 7) * (n >> 3) + (k >> 3); }
 // tile t of the upper triangle (ti <= tj) of n x n tiles, taken in bands of BAND columns, row by row within a band
 template <int BAND> __device__ __forceinline__ void sym_tile(int t, int n, int& ti, int& tj) {
   int b = (int)((sqrtf(8.f * t + 1.f) - 1.f) * (0.5f / BAND));     // column c starts at tile c (c + 1) / 2
@@ -469,37 +469,41 @@ template <int BAND> __device__ __forceinline__ void sym_tile(int t, int n, int& 
 template <int PHASE, bool last, class C>
 __global__ __launch_bounds__(C::NT) void orth_product_kernel(OrthHead h, OrthOut o, float ca, float cb, float cc, int flip) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int block = xcd_block();
   // (asked for together: one after the other they are a miss each)
-  asm volatile("" ::"s"(h.n), "s"(h.ws), "s"(h.first[1]), "s"(h.first[2]), "s"(h.first[3]), "s"(h.g[0].rp), "s"(h.g[0].cp), "s"(h.g[0].ws),
-               "s"(h.g[1].rp), "s"(h.g[1].ws), "s"(h.g[2].rp), "s"(h.g[2].ws), "s"(h.g[3].rp), "s"(h.g[3].ws));
-  int s = 0, first = 0;
-  struct { int r, c, rp, cp; int64_t ws; } G = {h.g[0].r, h.g[0].c, h.g[0].rp, h.g[0].cp, h.g[0].ws};
+  const int blocks = gridDim.x;
+  asm volatile("" ::"s"(h.n), "s"(h.spread), "s"(blocks), "s"(h.ws), "s"(h.first[1]), "s"(h.first[2]), "s"(h.first[3]), "s"(h.g[0].rp),
+               "s"(h.g[0].cp), "s"(h.g[0].batch), "s"(h.g[0].ws), "s"(h.g[1].rp), "s"(h.g[1].cp), "s"(h.g[1].batch), "s"(h.g[1].ws), "s"(h.g[2].rp),
+               "s"(h.g[2].cp), "s"(h.g[2].batch), "s"(h.g[2].ws), "s"(h.g[3].rp), "s"(h.g[3].cp), "s"(h.g[3].batch), "s"(h.g[3].ws));
+  const int block = h.spread ? (int)blockIdx.x : xcd_block(blockIdx.x, blocks);
+  int s = 0, first = 0, next = h.first[1];
+  struct { int r, c, rp, cp, batch; int64_t ws; } G = {h.g[0].r, h.g[0].c, h.g[0].rp, h.g[0].cp, h.g[0].batch, h.g[0].ws};
   if (h.n == 0) {
     const int* const all = PHASE == kApply ? h.args->full0 : h.args->sym0;
-    s = find_item(all, block); first = all[s];
+    s = find_item(all, block); first = all[s]; next = s + 1 < kOrthMax ? all[s + 1] : INT32_MAX;
     const OrthGeom& g = h.args->g[s];
-    G.r = g.r; G.c = g.c; G.rp = g.rp; G.cp = g.cp; G.ws = g.ws;
+    G.r = g.r; G.c = g.c; G.rp = g.rp; G.cp = g.cp; G.batch = g.batch; G.ws = g.ws;
   } else {
 #pragma unroll
     for (int k = 1; k < kHead; ++k) {
       const bool is = block >= h.first[k];
-      s = is ? k : s; first = is ? h.first[k] : first;
+      s = is ? k : s; first = is ? h.first[k] : first; next = is ? (k + 1 < kHead ? h.first[k + 1] : INT32_MAX) : next;
       G.r = is ? h.g[k].r : G.r; G.c = is ? h.g[k].c : G.c; G.rp = is ? h.g[k].rp : G.rp; G.cp = is ? h.g[k].cp : G.cp;
-      G.ws = is ? h.g[k].ws : G.ws;
+      G.batch = is ? h.g[k].batch : G.batch; G.ws = is ? h.g[k].ws : G.ws;
     }
   }
-  const int nti = (G.rp + C::T - 1) / C::T;
+  if (next == INT32_MAX) next = blocks;
+  const int nti = (G.rp + C::T - 1) / C::T, tile = h.spread ? xcd_block(block - first, next - first) : block - first;
   int mat, ti, tj;
   if (PHASE == kApply) {
-    const int ntj = (G.cp + C::T - 1) / C::T, k = block - first, t = k % (nti * ntj), band = t / (C::BAND * ntj);
+    const int ntj = (G.cp + C::T - 1) / C::T, t = tile % (nti * ntj), band = t / (C::BAND * ntj);
     const int h = nti - band * C::BAND < C::BAND ? nti - band * C::BAND : C::BAND, q = t - band * C::BAND * ntj;
-    mat = k / (nti * ntj); ti = band * C::BAND + q % h; tj = q / h;
+    mat = tile / (nti * ntj); ti = band * C::BAND + q % h; tj = q / h;
   } else {
-    const int per = nti * (nti + 1) / 2, k = block - first;
-    mat = k / per;
-    sym_tile<C::BAND>(k % per, nti, ti, tj);
+    const int per = nti * (nti + 1) / 2;
+    mat = tile / per;
+    sym_tile<C::BAND>(tile % per, nti, ti, tj);
   }
+  if (mat >= G.batch) return;        // what rounds the geometry's workgroups up
   const OrthPlanes P = orth_planes(G.rp, G.cp, C::SPLIT);
   _Float16* W = (_Float16*)(h.ws + G.ws) + mat * P.total;
   const int64_t yh = flip ? P.h[1] : P.h[0], yl = flip ? P.l[1] : P.l[0];
@@ -994,12 +998,20 @@ static int orth_plan(OrthArgs& a, int kind, OrthPlan& p) {
     return SNR_OK;
   }
   a.n_geom = 0;
+  for (int s = 0; s < a.n_items; ++s) {      // the sizes there are, longest K first: what takes longest begins first
+    const OrthIo& io = a.io[s];
+    const int r = io.m < io.n ? io.m : io.n, c = io.m < io.n ? io.n : io.m;
+    int k = 0;
+    while (k < a.n_geom && (a.g[k].c > c || (a.g[k].c == c && a.g[k].r > r))) ++k;
+    if (k < a.n_geom && a.g[k].c == c && a.g[k].r == r) continue;
+    for (int q = a.n_geom++; q > k; --q) a.g[q] = a.g[q - 1];
+    a.g[k] = OrthGeom{r, c, (r + kPad - 1) / kPad * kPad, (c + kPad - 1) / kPad * kPad, 0, 0, 0};
+  }
   for (int s = 0; s < a.n_items; ++s) {
     OrthIo& io = a.io[s];
     const int r = io.m < io.n ? io.m : io.n, c = io.m < io.n ? io.n : io.m;
     int k = 0;
-    while (k < a.n_geom && (a.g[k].r != r || a.g[k].c != c)) ++k;
-    if (k == a.n_geom) a.g[a.n_geom++] = OrthGeom{r, c, (r + kPad - 1) / kPad * kPad, (c + kPad - 1) / kPad * kPad, 0, 0, 0};
+    while (a.g[k].r != r || a.g[k].c != c) ++k;
     OrthGeom& g = a.g[k];
     io.geom = k; io.mat0 = g.batch; g.batch += io.batch;
     const int64_t n = ((int64_t)io.m * io.n + 8191) / 8192;
@@ -1020,7 +1032,7 @@ static int orth_plan(OrthArgs& a, int kind, OrthPlan& p) {
     OrthGeom& g = a.g[s];
     g.ws = off; off += (int64_t)g.batch * orth_planes(g.rp, g.cp, split).total * 2;
     a.sym0[s] = (int)p.sym; a.full0[s] = (int)p.full;
-    p.sym += sym_tiles(g, p.ts); p.full += full_tiles(g, p.tf);
+    p.sym += (sym_tiles(g, p.ts) + 7) / 8 * 8; p.full += (full_tiles(g, p.tf) + 7) / 8 * 8;
   }
   const int64_t at_part = align256(off);     // the planes come first: on 256 bytes
   a.part = (double*)(a.ws + at_part);
@@ -1035,6 +1047,7 @@ static OrthHead orth_head(const OrthArgs& a, const OrthArgs* in_ws, const int* f
   OrthHead h{};
   h.args = in_ws; h.ws = a.ws;
   h.n = a.n_geom <= kHead ? a.n_geom : 0;
+  h.spread = a.g[0].c >= 2 * a.g[a.n_geom - 1].c;
   for (int k = 0; k < kHead; ++k) { h.first[k] = k < a.n_geom ? first[k] : INT32_MAX; h.g[k] = a.g[k]; }
   return h;
 }
