@@ -323,7 +323,7 @@ template <int T_, int WI_, int WJ_, bool SPLIT_, int STAGES_, int BK_> struct Ti
   // where 16-byte chunk c of row r lies in a slice's plane
   static __host__ __device__ constexpr int swz(int r, int c) { return r * RB + ((c ^ (BK == 64 ? (r >> 1) & 7 : (r >> 2) & 3)) << 4); }
   // ... and, in Apply's Q slice, chunk c of row k: the 64 B that a group of 16 lanes reads of four rows fall on different banks
-  static __host__ __device__ constexpr int swzt(int k, int c) { return k * 2 * T + ((c ^ (T % 128 == 0 ? (k & 3) << 2 : (k >> 1 & 1) << 2)) << 4); }
+  static __host__ __device__ constexpr int swzt(int k, int c) { return k * 2 * T + ((c ^ (T % 128 == 0 ? (k & 3) << 2 : T > 32 ? (k >> 1 & 1) << 2 : 0)) << 4); }
   static constexpr int EPI = NW * 32 * 36 * 4;                    // epilogue: a 32 x 36 fp32 block a wave
 };
 
@@ -945,6 +945,8 @@ static int kind_of(int precision, int64_t m, int64_t n) {
   return split ? kSplit : kHalf;
 }
 
+using S32 = TileCfg<32, 1, 1, true, 4, 64>;
+using H32 = TileCfg<32, 1, 1, false, 4, 64>;
 using S64 = TileCfg<64, 2, 2, true, 2, 64>;
 using S128 = TileCfg<128, 4, 4, true, 2, 64>;
 using H64 = TileCfg<64, 2, 2, false, 3, 64>;
@@ -963,28 +965,33 @@ struct OrthPlan { int ts, tf; int64_t sym, full, chunk, split, bytes; OrthArgs* 
 static int64_t sym_tiles(const OrthGeom& g, int T) { const int64_t t = (g.rp + T - 1) / T; return g.batch * (t * (t + 1) / 2); }
 static int64_t full_tiles(const OrthGeom& g, int T) { return (int64_t)g.batch * ((g.rp + T - 1) / T) * ((g.cp + T - 1) / T); }
 
-// Tiles of 64, 128 and, for fp16 products, 192 (symmetric) or 256 (B Y).  A larger one reads less per product, but 128 and above have a
-// compute unit to themselves and idle ones are worth more: 128 from half the chip on.  Us a product at 64 / 128, fp16: symmetric,
-// 2048^2 (136 tiles of 128): 24 / 22, 4 x 1024^2 (144): 16 / 15, 3 x 1024^2 (108): 12 / 14; B Y, 1024 x 4096: 23 / 21, 1400^2: 17 / 20.  fp32
-// (no larger tile fits LDS twice): symmetric, 2048^2: 53 / 44, 1400^2: 21 / 29; B Y, 2048^2: 67 / 59, 3 x 1024^2: 34 / 30.
-static int pick_tile(int64_t n128) { return n128 >= cu_count() / 2 ? 128 : 64; }
+// Tiles of 32, 64, 128 and, for fp16 products, 192 (symmetric) or 256 (B Y).  A larger one reads less per product, but idle compute units are
+// worth more: 64 from 3 / 8 of the chip on, 128, which has a compute unit to itself, from half of it on.  A tile of 32 is one wave's.  Us a
+// call with / without 32 (tiles of 64 a symmetric product, B Y): fp32, 256 x 8000 (10, 500) 282 / 452, 256^2 (10, 16) 88 / 103, 512^2 (36, 64)
+// 114 / 142, 333 x 1000 (21, 96) x 4 (84, 384) 160 / 175, 2 x 512^2 (72, 128) 132 / 144; fp16 172 / 219, 72 / 80, 82 / 95, 114 / 120, 91 / 97; with
+// 32 everywhere 1024^2 (136, 256) and 14 x 256^2 (140, 224) are slower, B Y by a third.  Us a product at 64 / 128, fp16: symmetric, 2048^2
+// (136 tiles of 128): 24 / 22, 4 x 1024^2 (144): 16 / 15, 3 x 1024^2 (108): 12 / 14; B Y, 1024 x 4096: 23 / 21, 1400^2: 17 / 20.  fp32 (no
+// larger tile fits LDS twice): symmetric, 2048^2: 53 / 44, 1400^2: 21 / 29; B Y, 2048^2: 67 / 59, 3 x 1024^2: 34 / 30.
+static int pick_tile(int64_t n64, int64_t n128) { return 8 * n64 <= 3 * cu_count() ? 32 : n128 >= cu_count() / 2 ? 128 : 64; }
 // 128 or 192: a round of tiles (one a compute unit) takes as long as a tile's rows take to come in, the products of the whole chip as long
 // as its power allows, whichever is more; and every round after the first has an epilogue that nothing hides.  Us at 128 / 192: 4096^2
 // (528 / 253 tiles): 105 / 81, 2048^2 (136 / 66): 22 / 32, 13 x 1024^2 (468 / 273): 27 / 38, 2 x 2048 x 3000 (272 / 132): 50 / 42, 3 x 2048^2
 // (408 / 198): 40 / 38, 5 x 1500^2 (390 / 180): 32 / 30.
-static int pick_sym(int64_t n128, int64_t n192) {
+static int pick_sym(int64_t n64, int64_t n128, int64_t n192) {
   const int64_t cus = cu_count();
   auto cost = [&](double T, int64_t n, double slower) {
     const double rounds = (double)((n + cus - 1) / cus);
     return fmax(rounds * T * slower, (double)n * T * T / (99.0 * (double)cus)) * (0.9 + 0.1 * rounds);
   };
-  return pick_tile(n128) == 128 && cost(192, n192, 1.13) < cost(128, n128, 1.0) ? 192 : pick_tile(n128);
+  const int T = pick_tile(n64, n128);
+  return T == 128 && cost(192, n192, 1.13) < cost(128, n128, 1.0) ? 192 : T;
 }
 // 128 or 256: 256 where its rounds are more than three quarters full.  Us at 128 / 256: 4096^2 (256 tiles of 256): 144 / 133, 2048 x 7000
 // (224): 82 / 77, 3500^2 (196): 120 / 106, 3 x 2048^2 (192): 73 / 77, 12 x 512 x 2048 (192): 34 / 40, 5 x 1500^2 (180): 58 / 61.
-static int pick_full(int64_t n128, int64_t n256) {
+static int pick_full(int64_t n64, int64_t n128, int64_t n256) {
   const int64_t cus = cu_count(), room = (n256 + cus - 1) / cus * cus;
-  return pick_tile(n128) == 128 && 4 * n256 > 3 * room ? 256 : pick_tile(n128);
+  const int T = pick_tile(n64, n128);
+  return T == 128 && 4 * n256 > 3 * room ? 256 : T;
 }
 
 static int orth_plan(OrthArgs& a, int kind, OrthPlan& p) {
@@ -1021,14 +1028,12 @@ static int orth_plan(OrthArgs& a, int kind, OrthPlan& p) {
     a.split0[s] = (int)p.split; p.split += (int64_t)io.batch * (g.rp / kPad) * (g.cp / kPad);
     if (p.chunk > kMaxBlocks || p.split > kMaxBlocks) return SNR_ERR_SHAPE;
   }
-  int64_t ns[2] = {0, 0}, nf[2] = {0, 0};
-  for (int s = 0; s < a.n_geom; ++s) {
-    ns[0] += sym_tiles(a.g[s], 128); ns[1] += sym_tiles(a.g[s], 192);
-    nf[0] += full_tiles(a.g[s], 128); nf[1] += full_tiles(a.g[s], 256);
-  }
-  p.ts = split ? pick_tile(ns[0]) : pick_sym(ns[0], ns[1]);
-  p.tf = split ? pick_tile(nf[0]) : pick_full(nf[0], nf[1]);
-  for (int s = 0; s < a.n_geom; ++s) {       // (no more tiles than the split's: one holds 64 x 64 or more)
+  int64_t ns[3] = {}, nf[3] = {};
+  for (int s = 0; s < a.n_geom; ++s)
+    for (int k = 0; k < 3; ++k) { ns[k] += sym_tiles(a.g[s], k < 2 ? 64 << k : 192); nf[k] += full_tiles(a.g[s], 64 << k); }
+  p.ts = split ? pick_tile(ns[0], ns[1]) : pick_sym(ns[0], ns[1], ns[2]);
+  p.tf = split ? pick_tile(nf[0], nf[1]) : pick_full(nf[0], nf[1], nf[2]);
+  for (int s = 0; s < a.n_geom; ++s) {       // (no more tiles than the split's where there are many: one holds 64 x 64 or more)
     OrthGeom& g = a.g[s];
     g.ws = off; off += (int64_t)g.batch * orth_planes(g.rp, g.cp, split).total * 2;
     a.sym0[s] = (int)p.sym; a.full0[s] = (int)p.full;
@@ -1059,8 +1064,11 @@ static void launch(const OrthHead& a, const OrthOut& o, int64_t n, float ca, flo
 template <int PHASE, bool last>
 static void launch_tile(bool split, int T, const OrthHead& a, const OrthOut& o, int64_t n, float ca, float cb, float cc, int flip, hipStream_t st) {
   if (split) {
-    if (T == 64) launch<PHASE, last, S64>(a, o, n, ca, cb, cc, flip, st);
+    if (T == 32) launch<PHASE, last, S32>(a, o, n, ca, cb, cc, flip, st);
+    else if (T == 64) launch<PHASE, last, S64>(a, o, n, ca, cb, cc, flip, st);
     else launch<PHASE, last, S128>(a, o, n, ca, cb, cc, flip, st);
+  } else if (T == 32) {
+    launch<PHASE, last, H32>(a, o, n, ca, cb, cc, flip, st);
   } else if (T == 64) {
     launch<PHASE, last, H64>(a, o, n, ca, cb, cc, flip, st);
   } else if (T == 128) {
