@@ -15,15 +15,15 @@ LIB_PATH = os.path.join(LIB_DIR, "libspinnerf_hip.so")
 
 # (source, extra flags).  render_ops is built without FMA contraction so its elementwise fp32
 # arithmetic rounds like the reference's separate torch ops.
-# The two fused-MLP sources also keep their gfx950 listing (lib/<name>.gfx950.s): their LDS reads are inline
-# asm with hand-counted waits, and tools/check_lds_asm.py verifies on the listing that nothing touches a
-# destination register before its wait — build() fails if it does.
+# The two fused-MLP sources and muon.hip also keep their gfx950 listing (lib/<name>.gfx950.s): their LDS reads or LDS-DMA
+# are inline asm with hand-counted waits, and tools/check_lds_asm.py verifies on the listing that nothing touches a
+# destination register before its wait and that no scalar base is read too early — build() fails if it does.
 SOURCES = [
     ("mlp_fwd.hip", ["-save-temps=obj"]),
     ("mlp_bwd.hip", ["-save-temps=obj"]),
     ("render_ops.hip", ["-ffp-contract=off"]),
     ("adam_pack.hip", ["-ffp-contract=off"]),    # Adam + weight pack in one kernel: must round like render_ops' adam_kernel
-    ("muon.hip", []),
+    ("muon.hip", ["-save-temps=obj", "-Wno-inline-asm"]),   # (its asm names m0 as clobbered: reserved, but written)
     ("hashgrid.hip", ["-munsafe-fp-atomics"]),   # table gradients: hardware global_atomic_add_f32, no CAS loops
     ("prof.cpp", ["-x", "hip"]),
     ("fused.cpp", ["-x", "hip"]),                # render_rays as one call: launch order only, no kernels
@@ -58,11 +58,13 @@ def _keep_listings(verbose):
     listings = sorted(os.path.join(LIB_DIR, f) for f in os.listdir(LIB_DIR) if f.endswith(".gfx950.s"))
     if listings:
         tool = os.path.join(os.path.dirname(HERE), "tools", "check_lds_asm.py")
-        r = subprocess.run([sys.executable, tool] + listings, capture_output=True, text=True)
+        own = [p for p in listings if os.path.basename(p).startswith("muon.")]
+        r = subprocess.run([sys.executable, tool] + [p for p in listings if p not in own] + (["--own"] + own if own else []),
+                           capture_output=True, text=True)
         if verbose or r.returncode:
             print(r.stdout.strip()[-2000:], flush=True)
         if r.returncode:
-            raise RuntimeError("check_lds_asm.py: an asm LDS read is consumed before its wait (or no kernel was recognised)")
+            raise RuntimeError("check_lds_asm.py: an asm LDS read is consumed before its wait, a scalar base is read too early (or no kernel was recognised)")
         # register spills of the weight-gradient kernels must stay out of their tile loops (tools/check_spills.py: no scratch_* /
         # v_writelane / v_readlane inside an innermost loop that contains MFMAs; the chain kernels' only MFMA loop is the pass
         # loop around the whole unrolled network, so the criterion does not apply to them: reported, not gated)

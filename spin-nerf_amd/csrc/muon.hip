@@ -327,26 +327,55 @@ template <int T_, int WI_, int WJ_, bool SPLIT_, int STAGES_, int BK_> struct Ti
   static constexpr int EPI = NW * 32 * 36 * 4;                    // epilogue: a 32 x 36 fp32 block a wave
 };
 
-// 16 bytes a lane from base + off straight to LDS at dst + 16 lane.  In asm, as the compiler cannot tell which LDS reads such a load
-// concerns and waits for all of them; the waits are landed()'s.  It has no register to be overwritten, and it is counted in order
-// with every other load, so that the compiler's own waits only get stricter.
-__device__ __forceinline__ void dma16(unsigned dst, const _Float16* base, unsigned off) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(off), "s"(base) : "memory");
-}
 __device__ __forceinline__ unsigned lds_at(const char* p) { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p; }
 
-// a slice past the end is one 16-byte piece again and again: the number of loads in flight stays what the waits count on
+// A slice, 16 bytes a lane and load, from base + off straight to LDS: a wave's pieces lie NW KB apart, plane after plane.  In asm, as
+// the compiler cannot tell which LDS reads such a load concerns and waits for all of them; the waits are landed()'s.  There is no
+// register to be overwritten, and the loads are counted in order with every other one, so that the compiler's own waits only get
+// stricter.  Nor does the compiler see into it for hazards: a VALU write of a base (a readfirstlane, a spilled SGPR read back) has to be
+// five wait states away, whatever it puts in front: s_mov and the four of s_nop 3, once for the whole slice (at every load: 4 x 1000 x
+// 333 fp16 161 -> 169 us, 2048 x 8192 bf16 834 -> 860); tools/check_lds_asm.py --own holds the listing to it.  m0 needs one.
+// A slice past the end is one 16-byte piece again and again: the number of loads in flight stays what the waits count on.
+#define SNR_DMA_FIRST "s_mov_b32 m0, %[d]\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %[x0], %[p0]"
+#define SNR_DMA(off, base) "\n\ts_add_u32 m0, m0, %[s]\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %[" off "], %[" base "]"
 template <class C>
 __device__ __forceinline__ void fetch_slice(unsigned dst, const _Float16* const (&src)[4], const unsigned (&voff)[2][C::PER], int k, int n, int64_t ldq, int wave) {
+  static_assert(C::SECT == C::PER * C::NW * 1024, "a plane's pieces and the next one's first are as far apart");
   const int k0 = k < n ? k * C::BK : 0;
-  const unsigned keep = k < n ? ~0u : 0u;
+  const unsigned keep = k < n ? ~0u : 0u, d = dst + wave * 1024;
+  const _Float16 *p0 = src[0] + k0, *q0 = src[1] + k0 * ldq, *p1 = src[2] + k0, *q1 = src[3] + k0 * ldq;   // hi of P and Q, lo
+  unsigned x[4], y[4];
 #pragma unroll
-  for (int p = 0; p < (C::SPLIT ? 4 : 2); ++p) {
-    const _Float16* base = src[p] + (p & 1 ? k0 * ldq : k0);
-#pragma unroll
-    for (int q = 0; q < C::PER; ++q) dma16(dst + p * C::SECT + (wave + q * C::NW) * 1024, base, voff[p & 1][q] & keep);
+  for (int q = 0; q < 4; ++q) { x[q] = voff[0][q < C::PER ? q : 0] & keep; y[q] = voff[1][q < C::PER ? q : 0] & keep; }
+#define SNR_DMA_ARGS(...) [d] "s"(d), [s] "n"(C::NW * 1024), [p0] "s"(p0), [q0] "s"(q0), __VA_ARGS__ : "memory", "m0", "scc"
+  if constexpr (C::SPLIT && C::PER == 1)
+    asm volatile(SNR_DMA_FIRST SNR_DMA("y0", "q0") SNR_DMA("x0", "p1") SNR_DMA("y0", "q1")
+                 ::SNR_DMA_ARGS([p1] "s"(p1), [q1] "s"(q1), [x0] "v"(x[0]), [y0] "v"(y[0])));
+  else if constexpr (C::SPLIT && C::PER == 2)
+    asm volatile(SNR_DMA_FIRST SNR_DMA("x1", "p0") SNR_DMA("y0", "q0") SNR_DMA("y1", "q0")
+                 SNR_DMA("x0", "p1") SNR_DMA("x1", "p1") SNR_DMA("y0", "q1") SNR_DMA("y1", "q1")
+                 ::SNR_DMA_ARGS([p1] "s"(p1), [q1] "s"(q1), [x0] "v"(x[0]), [x1] "v"(x[1]), [y0] "v"(y[0]), [y1] "v"(y[1])));
+  else if constexpr (C::SPLIT && C::PER == 4)
+    asm volatile(SNR_DMA_FIRST SNR_DMA("x1", "p0") SNR_DMA("x2", "p0") SNR_DMA("x3", "p0")
+                 SNR_DMA("y0", "q0") SNR_DMA("y1", "q0") SNR_DMA("y2", "q0") SNR_DMA("y3", "q0")
+                 SNR_DMA("x0", "p1") SNR_DMA("x1", "p1") SNR_DMA("x2", "p1") SNR_DMA("x3", "p1")
+                 SNR_DMA("y0", "q1") SNR_DMA("y1", "q1") SNR_DMA("y2", "q1") SNR_DMA("y3", "q1")
+                 ::SNR_DMA_ARGS([p1] "s"(p1), [q1] "s"(q1), [x0] "v"(x[0]), [x1] "v"(x[1]), [x2] "v"(x[2]), [x3] "v"(x[3]),
+                                [y0] "v"(y[0]), [y1] "v"(y[1]), [y2] "v"(y[2]), [y3] "v"(y[3])));
+  else if constexpr (C::PER == 2)
+    asm volatile(SNR_DMA_FIRST SNR_DMA("x1", "p0") SNR_DMA("y0", "q0") SNR_DMA("y1", "q0")
+                 ::SNR_DMA_ARGS([x0] "v"(x[0]), [x1] "v"(x[1]), [y0] "v"(y[0]), [y1] "v"(y[1])));
+  else {
+    static_assert(!C::SPLIT && C::PER == 4, "a slice's loads are written out for these");
+    asm volatile(SNR_DMA_FIRST SNR_DMA("x1", "p0") SNR_DMA("x2", "p0") SNR_DMA("x3", "p0")
+                 SNR_DMA("y0", "q0") SNR_DMA("y1", "q0") SNR_DMA("y2", "q0") SNR_DMA("y3", "q0")
+                 ::SNR_DMA_ARGS([x0] "v"(x[0]), [x1] "v"(x[1]), [x2] "v"(x[2]), [x3] "v"(x[3]),
+                                [y0] "v"(y[0]), [y1] "v"(y[1]), [y2] "v"(y[2]), [y3] "v"(y[3])));
   }
+#undef SNR_DMA_ARGS
 }
+#undef SNR_DMA_FIRST
+#undef SNR_DMA
 
 // one slice: the fragments of the next 16 of K are read while those of this 16 are multiplied (sched_barrier keeps the compiler from
 // moving the reads back to their use: a wave alone on its SIMD would wait out LDS's latency eight times a slice)

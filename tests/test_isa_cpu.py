@@ -140,3 +140,27 @@ def test_spill_checker_tells_a_tile_loop_from_the_prologue(tmp_path):
         assert r.returncode == 0, r.stdout
         assert "mlp_wgrad_pair_kernel" in r.stdout and "(in an innermost MFMA loop: 0)" in r.stdout
 
+
+def test_checker_wants_five_wait_states_in_front_of_a_scalar_base(tmp_path):
+    first = "        v_readfirstlane_b32 %s, v0\n"
+    dma = "        ;;#ASMSTART\n        s_mov_b32 m0, s5\n        s_nop %d\n        global_load_lds_dwordx4 v9, s[6:7]\n        ;;#ASMEND\n"
+    assert chk.check(_listing(tmp_path, first % "s6" + dma % 0)) == 1      # two in between
+    assert chk.check(_listing(tmp_path, first % "s7" + dma % 2)) == 1      # four
+    assert chk.check(_listing(tmp_path, first % "s7" + dma % 3)) == 0      # five
+    assert chk.check(_listing(tmp_path, first % "s6" + "        s_add_u32 s8, s8, 1\n" * 3 + dma % 0)) == 0
+    assert chk.check(_listing(tmp_path, first % "s9" + dma % 0)) == 0      # another register
+    # ... inside the block, whatever the compiler has put in front of it this time
+    assert chk.check(_listing(tmp_path, "        s_nop 7\n" + dma % 0), own=True) == 1
+    assert chk.check(_listing(tmp_path, dma % 3), own=True) == 0
+    # written by the compiler, which keeps the distance itself; and an address in vector registers alone
+    assert chk.check(_listing(tmp_path, "        s_nop 7\n        global_load_lds_dwordx4 v9, s[4:5]\n"), own=True) == 0
+    assert chk.check(_listing(tmp_path, "        s_nop 7\n        ;;#ASMSTART\n        global_load_lds_dwordx4 v[8:9], off\n        ;;#ASMEND\n"), own=True) == 0
+
+
+def test_the_orthogonalise_kernels_wait_inside_their_asm():
+    """their LDS-DMA is inline asm with a scalar base, where the compiler's hazard recogniser does not look"""
+    lst = os.path.join(ROOT, "spin-nerf_amd", "lib", "muon.gfx950.s")
+    if not os.path.exists(lst):
+        pytest.skip("no device listing (run __graft_entry__.build() first)")
+    assert open(lst).read().count("global_load_lds_dwordx4") > 100
+    assert chk.check(lst, own=True) == 0

@@ -13,7 +13,12 @@ Second check, for the MFMAs issued from inline asm (the layer-pair weight-gradie
 recogniser does not look into asm, so a VALU instruction that writes one of an asm MFMA's source registers must be at
 least two wait states in front of it (an `s_nop N` counts N + 1; every other instruction counts one).
 
-  python tools/check_lds_asm.py file.s   -> exit status 1 on a violation
+Third check, for vector-memory instructions in inline asm whose address has a scalar base: a VALU instruction that writes an SGPR
+(v_readfirstlane, a spilled SGPR's v_readlane) must be five wait states in front of a vector-memory instruction that reads it.
+Behind `--own` the five have to be inside the asm block itself, as what stands in front of it is the compiler's choice, anew in
+every build; the layer-pair kernel, which spreads m0 and load over blocks of their own, is held to what its listing says.
+
+  python tools/check_lds_asm.py file.s [file.s ...] [--own file.s ...]   -> exit status 1 on a violation
 """
 import re, sys
 
@@ -29,14 +34,25 @@ def regs(text):
     return out
 
 unverified = [0]  # uses of an asm global load with a branch between load and use: outside the straight-line model
+VMEM = re.compile(r"(global|scratch|buffer|flat)_")
+
+def sregs(text):
+    out = set()
+    for m in re.finditer(r"\bs\[(\d+):(\d+)\]|\bs(\d+)\b", text):
+        out.update(range(int(m.group(1)), int(m.group(2)) + 1) if m.group(1) else [int(m.group(3))])
+    if re.search(r"\bvcc\b", text):
+        out.add("vcc")
+    return out
+
 n_kernels = [0]   # kernels seen by check() so far: a listing in which none is recognised is an error, not a pass
 
 
-def check(path):
+def check(path, own=False):
     bad = 0
     kernel, pending, issued, in_asm = None, [], 0, False
     vpending = []   # asm global loads: [destination registers, line, vector-memory LOADS issued behind it]
     recent = []     # the last instructions of the kernel, youngest last: (line, code)
+    inside = 0      # instructions of the asm block so far
     for ln, line in enumerate(open(path), 1):
         s = line.strip()
         m = re.match(r"(_Z\w+):", s)          # (the label line carries a trailing `; @name` comment)
@@ -45,7 +61,7 @@ def check(path):
             n_kernels[0] += 1
             continue
         if s.startswith(";;#ASMSTART"):
-            in_asm = True; continue
+            in_asm, inside = True, 0; continue
         if s.startswith(";;#ASMEND"):
             in_asm = False; continue
         if not s or s.startswith((";", ".", "//")) or kernel is None:
@@ -66,7 +82,24 @@ def check(path):
                     print(f"{path}:{ln}: {kernel[:60]}: asm `{code[:50]}` reads a register `{pc[:50]}` (line {l0}) wrote {ws} wait states earlier")
                     bad += 1
                 ws += 1
-        recent = (recent + [(ln, code)])[-4:]
+        if in_asm and VMEM.match(code):
+            base, ws = sregs(code.split(None, 1)[1]), 0
+            for k, (l0, pc) in enumerate(reversed(recent)):
+                if ws >= 5 or not base:
+                    break
+                if own and k >= inside:
+                    print(f"{path}:{ln}: {kernel[:60]}: asm `{code[:50]}` reads a scalar base with {ws} wait states of its own block in front: five are needed")
+                    bad += 1
+                    break
+                if pc.startswith("s_nop"):
+                    ws += int(pc.split()[1]) + 1
+                    continue
+                if pc.startswith("v_") and sregs(pc.split(None, 1)[1].split(",")[0]) & base:
+                    print(f"{path}:{ln}: {kernel[:60]}: asm `{code[:50]}` reads a scalar base that `{pc[:50]}` (line {l0}) wrote {ws} wait states earlier")
+                    bad += 1
+                ws += 1
+        inside += 1
+        recent = (recent + [(ln, code)])[-8:]
         if in_asm and code.startswith("ds_read"):
             dst = regs(code.split(",")[0])
             issued += 1
@@ -117,6 +150,7 @@ def check(path):
     return bad
 
 if __name__ == "__main__":
-    n = sum(check(p) for p in sys.argv[1:])
+    at = sys.argv.index("--own") if "--own" in sys.argv else len(sys.argv)
+    n = sum(check(p) for p in sys.argv[1:at]) + sum(check(p, own=True) for p in sys.argv[at + 1:])
     print("violations:", n, "kernels checked:", n_kernels[0], "global-load uses behind control flow (not checkable):", unverified[0])
     sys.exit(1 if n or not n_kernels[0] else 0)
