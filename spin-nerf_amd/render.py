@@ -323,7 +323,10 @@ def ndc_rays(H, W, focal, near, rays_o, rays_d):
 def _load_per_layer_adam(optimizer, osd, nets):
     """Load a reference-format optimizer state (one entry per layer tensor, coarse network first) into the Adam over
     the networks' flat parameters.  Raises when the layouts do not correspond — a resumed run must not silently
-    restart its moments, bias correction and learning-rate decay."""
+    restart its moments, bias correction and learning-rate decay.
+
+    A state that RenderTrainer(muon=...) wrote is kept for such a trainer, under `momentum_buffer` in place of `exp_avg`: neither
+    RenderTrainer without muon nor torch.optim.Adam itself steps from that."""
     st = osd.get('state', {})
     n_params = sum(len(n.param_views()) for n in nets)
     groups = osd.get('param_groups') or [{}]
@@ -336,9 +339,10 @@ def _load_per_layer_adam(optimizer, osd, nets):
     if not st:
         return
     moments = [(torch.zeros_like(n.flat.data), torch.zeros_like(n.flat.data)) for n in nets]
-    steps = scatter_per_layer_adam(st, nets, moments)
+    muon = any('momentum_buffer' in e for e in st.values())
+    steps = scatter_per_layer_adam(st, nets, moments, muon=muon)
     for n, (m, v), stp in zip(nets, moments, steps):
-        optimizer.state[n.flat] = {'step': torch.tensor(float(stp)), 'exp_avg': m, 'exp_avg_sq': v}
+        optimizer.state[n.flat] = {'step': torch.tensor(float(stp)), 'momentum_buffer' if muon else 'exp_avg': m, 'exp_avg_sq': v}
 
 
 def scatter_per_layer_adam(st, nets, moments, muon=False):
@@ -366,7 +370,7 @@ def scatter_per_layer_adam(st, nets, moments, muon=False):
                     raise RuntimeError(f"optimizer_state_dict has no Adam state for parameter {idx} ({name}): cannot resume the optimizer")
             elif ('momentum_buffer' in e) != (muon and name in n.hidden_matrices()):
                 raise RuntimeError(f"optimizer state of parameter {idx} ({name}): " + (
-                    "a momentum buffer, written by RenderTrainer(muon=...): resume with RenderTrainer(muon=...).load_checkpoint"
+                    "a momentum buffer, written by RenderTrainer(muon=...): only such a trainer resumes from it"
                     if 'momentum_buffer' in e else "Adam moments where RenderTrainer(muon=...) keeps a momentum buffer: load the networks' "
                     "weights alone and start the optimizer anew"))
             elif 'momentum_buffer' in e:

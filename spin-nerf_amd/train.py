@@ -86,18 +86,22 @@ class RenderTrainer:
         self._works[i] = dist.all_reduce(p.grad, op=dist.ReduceOp.SUM, group=self.pg, async_op=True)
 
     def _adopt(self, optimizer, start):
-        """continue from a torch.optim.Adam over the networks' flat parameters (create_nerf's return value)"""
+        """continue from a torch.optim.Adam over the networks' flat parameters (create_nerf's return value), which carries the state
+        of a checkpoint that RenderTrainer(muon=...) wrote under `momentum_buffer` in place of `exp_avg`"""
         st = optimizer.state
-        have = [n.flat in st and 'exp_avg' in st[n.flat] for n in self.nets]
-        if any(have) and self.muon is not None:
+        first, other = ('exp_avg', 'momentum_buffer') if self.muon is None else ('momentum_buffer', 'exp_avg')
+        have = [n.flat in st and first in st[n.flat] for n in self.nets]
+        if any(n.flat in st and other in st[n.flat] for n in self.nets):
             raise RuntimeError("the optimizer holds Adam state for the hidden matrices; RenderTrainer(muon=...) resumes its own checkpoints "
-                               "(load_checkpoint) or starts anew")
+                               "or starts anew" if self.muon is not None else
+                               "the optimizer holds momentum buffers for the hidden matrices, from a checkpoint of RenderTrainer(muon=...); "
+                               "only such a trainer resumes from it")
         if any(have) and not all(have):
-            raise RuntimeError("the optimizer holds Adam state for some of the networks only; cannot resume")
+            raise RuntimeError("the optimizer holds state for some of the networks only; cannot resume")
         if all(have) and self.nets:
             steps = []
             for i, n in enumerate(self.nets):
-                self.m[i].copy_(st[n.flat]['exp_avg']); self.v[i].copy_(st[n.flat]['exp_avg_sq'])
+                self.m[i].copy_(st[n.flat][first]); self.v[i].copy_(st[n.flat]['exp_avg_sq'])
                 steps.append(int(st[n.flat]['step']))
             if len(set(steps)) != 1:
                 raise RuntimeError(f"networks disagree on the Adam step count: {steps}")
