@@ -28,8 +28,8 @@ def img2mse(x, y):
 class RenderTrainer:
     def __init__(self, render_kwargs_train, lrate=5e-4, lrate_decay=250, world_size=1, process_group=None,
                  optimizer=None, start=None, graph=False, muon=None):
-        """``muon``: None = Adam on every parameter, like the reference; True or a dict of muon_step_'s settings (momentum, nesterov,
-        weight_decay, scale, steps, coefficients, eps, precision) = orthogonalised updates for the networks' hidden matrices
+        """``muon``: None = Adam on every parameter, like the reference; True or a dict of muon_step_'s settings (any of momentum,
+        nesterov, weight_decay, scale, steps, coefficients, eps, precision) = orthogonalised updates for the networks' hidden matrices
         (NeRF.hidden_matrices) and Adam for the rest, at one learning rate: scale defaults to "rms", whose steps are about Adam's size.
 
         ``optimizer`` / ``start`` = what create_nerf() returned: when it reloaded a checkpoint (run_nerf.py:448-462)
@@ -48,7 +48,9 @@ class RenderTrainer:
         self.m = [torch.zeros_like(n.flat.data) for n in self.nets]
         self.v = [torch.zeros_like(n.flat.data) for n in self.nets]
         self.muon = None              # else: the hidden matrices' parts of self.m are momentum buffers, those of self.v stay zero
-        if muon:
+        if not (muon is None or isinstance(muon, dict) or isinstance(muon, int) and muon in (0, 1)):
+            raise ValueError(f"RenderTrainer: muon must be True or a dict of settings (or None), got {muon!r}")
+        if isinstance(muon, dict) or muon:        # ({}: the defaults)
             self.muon = dict(momentum=0.95, nesterov=True, weight_decay=0.0, scale="rms", steps=5, coefficients=ops.NEWTON_SCHULZ,
                              eps=1e-7, precision="fp32")
             unknown = set(muon) - set(self.muon) if isinstance(muon, dict) else set()
