@@ -743,6 +743,9 @@ def _orth_args(name, steps, coefficients, eps, precision):
         raise ValueError(f"{name}: steps must be a whole number from 1 to 100, got {steps!r}")
     if not eps >= 1e-30:
         raise ValueError(f"{name}: eps must be at least 1e-30, got {eps!r}")
+    coefficients = tuple(coefficients)
+    if len(coefficients) != 3:
+        raise ValueError(f"{name}: expected three coefficients, got {coefficients!r}")
     a, b, c = (float(v) for v in coefficients)
     return int(steps), a, b, c, float(eps), _ORTH_PREC[precision]
 
@@ -752,6 +755,27 @@ def _orth_check(status, name, what):
         raise ValueError(f"{name}: the coefficients must keep singular values from [0, 1] below 8 over all steps, and |b l + c l^2| "
                          "below 64 for the squares l of all singular values on the way")
     check(status, what)
+
+
+def muon_settings(name, momentum, nesterov, weight_decay, scale, steps, coefficients, eps, precision):
+    """the settings of muon_step_ that do not change from step to step, checked on the host and in plain types"""
+    for what, v in (("momentum", momentum), ("weight_decay", weight_decay)):
+        try:
+            number = float(v) == float(v)
+        except (TypeError, ValueError):
+            number = False
+        if not number:
+            raise ValueError(f"{name}: {what} must be a number, got {v!r}")
+    if scale not in _MUON_SCALE:
+        raise ValueError(f"{name}: scale must be one of {sorted(_MUON_SCALE)}, got {scale!r}")
+    args = _orth_args(name, steps, coefficients, eps, precision)
+    # the library checks the coefficients ahead of its items: with one that is empty it answers without a launch
+    st = _lib.load().snr_muon_step_multi((_lib.MuonItem * 1)(), 1, 0.0, float(momentum), int(bool(nesterov)), float(weight_decay),
+                                         _MUON_SCALE[scale], *args[:5], 1.0, args[5], None, 256, None)
+    if st != _lib.ERR_NULL:
+        _orth_check(st, name, "snr_muon_step_multi")
+    return dict(momentum=float(momentum), nesterov=bool(nesterov), weight_decay=float(weight_decay), scale=scale, steps=args[0],
+                coefficients=args[1:4], eps=args[4], precision=precision)
 
 
 def orthogonalise(x, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, precision=None, out=None):

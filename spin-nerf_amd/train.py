@@ -56,7 +56,7 @@ class RenderTrainer:
             unknown = set(muon) - set(self.muon) if isinstance(muon, dict) else set()
             if unknown:
                 raise ValueError(f"RenderTrainer: muon has no settings {sorted(unknown)}; there are {sorted(self.muon)}")
-            self.muon.update(muon if isinstance(muon, dict) else {})
+            self.muon = ops.muon_settings("RenderTrainer(muon=...)", **dict(self.muon, **(muon if isinstance(muon, dict) else {})))
             bad = [type(n).__name__ for n in self.nets if not hasattr(n, "split_hidden")]
             if bad:
                 raise NotImplementedError(f"RenderTrainer: muon is for NeRF networks, whose hidden layers are matrices of their own; got {bad}")
