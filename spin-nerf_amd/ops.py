@@ -4,6 +4,7 @@ Every function here enqueues work on torch's current HIP stream through ``_lib``
 outputs/workspaces with torch's caching allocator; there is no eager/PyTorch fallback.
 """
 import torch
+import torch.autograd.forward_ad as _fwd
 
 from . import _lib
 from ._lib import check, f32c, ptr, stream
@@ -787,13 +788,15 @@ def orthogonalise(x, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, precision=No
     the matrix work (where the shorter side is above 64; below, it is "fp32"); default "fp16" for bf16 tensors (their own roundings
     are coarser) and "fp32" for the others.  A zero matrix gives zeros, one with a NaN or an infinity NaN throughout.  Any strides;
     sides and stack of at most 65536.  ``out`` (contiguous, may be x): where the result goes.  Not differentiable: an x that requires
-    grad is refused unless grad mode is off."""
+    grad is refused unless grad mode is off, and one with a forward-mode tangent always."""
     if not isinstance(x, torch.Tensor) or x.dim() < 2:
         raise ValueError(f"orthogonalise: expected a tensor [..., m, n], got {tuple(x.shape) if isinstance(x, torch.Tensor) else type(x).__name__}")
     if x.dtype not in _ORTH_TYPES:
         raise ValueError(f"orthogonalise: expected float32, float16 or bfloat16, got {x.dtype}")
     if torch.is_grad_enabled() and (x.requires_grad or (out is not None and out.requires_grad)):
         raise RuntimeError("orthogonalise has no backward pass: call it under torch.no_grad() or on x.detach()")
+    if getattr(_fwd, "_current_level", 0) >= 0 and any(t is not None and _fwd.unpack_dual(t).tangent is not None for t in (x, out)):
+        raise RuntimeError("orthogonalise has no forward-mode derivative: call it on the tensor that unpack_dual gives as primal")
     args = _orth_args("orthogonalise", steps, coefficients, eps, precision or ("fp16" if x.dtype == torch.bfloat16 else "fp32"))
     if not x.is_cuda:
         raise _lib.HipLibraryError("orthogonalise: the kernels need device (HIP) tensors; got a CPU tensor")
