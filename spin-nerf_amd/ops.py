@@ -669,7 +669,7 @@ def _rows(name, lists, read):
     lists = [list(x) for x in lists]
     if any(len(x) != len(lists[0]) for x in lists):
         raise ValueError(f"{name}: the lists differ in length: {[len(x) for x in lists]}")
-    rows, dev = list(zip(*lists)), None
+    rows, dev, f32 = list(zip(*lists)), None, torch.float32
     for i, row in enumerate(rows):
         first = row[0]
         shape = first.shape
@@ -681,7 +681,7 @@ def _rows(name, lists, read):
                 if dev is not None:
                     raise ValueError(f"{name}: expected a tensor on cuda:{dev}, got {t.device}")
                 dev = at
-            if t.dtype != torch.float32:
+            if t.dtype != f32:
                 raise ValueError(f"{name}: expected float32, got {t.dtype}")
             if t is not first and t.shape != shape:
                 raise ValueError(f"{name}: shapes of one item differ: {[tuple(u.shape) for u in row]}")
@@ -690,6 +690,10 @@ def _rows(name, lists, read):
                     raise ValueError(f"{name}: tensors that are written must be contiguous; got strides {t.stride()} for {tuple(t.shape)}")
                 rows[i] = rows[i][:k] + (t.contiguous(),) + rows[i][k + 1:]
     return rows, dev
+
+
+# what was written through raw pointers counts as modified in place, for autograd's saved tensors and a network's packed weights
+_modified = torch.autograd.graph.increment_version
 
 
 def _items(struct, values):
@@ -726,6 +730,7 @@ def adam_step_multi_(params, grads, exp_avgs, exp_avg_sqs, lr, step, beta1=0.9, 
     if st:
         _no_overlap("adam_step_multi_", rows, 1)
         check(st, "snr_adam_step_multi")
+    _modified([t for p, _, m, v in rows for t in (p, m, v)])
 
 
 # ----------------------------------------------------------------------------------------------
@@ -823,6 +828,7 @@ def orthogonalise(x, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, precision=No
             _orth_check(lib.snr_orthogonalise(ptr(y), dt, y.shape[0], m, n, y.stride(0), max(y.stride(1), n), ptr(res), m * n, n, *st, prec,
                                               ptr(ws), stream()), "orthogonalise", "snr_orthogonalise")
     if out is not None:
+        _modified(out)
         return out
     return res.reshape(x.mT.shape).mT if flip else res.reshape(x.shape)
 
@@ -876,3 +882,4 @@ def muon_step_(params, grads, momentum_buffers, lr, momentum=0.95, nesterov=True
     if st:
         _no_overlap("muon_step_", rows, 1)
         _orth_check(st, "muon_step_", "snr_muon_step_multi")
+    _modified([t for p, _, m in rows for t in (p, m)])
