@@ -3,6 +3,8 @@
 Every function here enqueues work on torch's current HIP stream through ``_lib`` and allocates its
 outputs/workspaces with torch's caching allocator; there is no eager/PyTorch fallback.
 """
+import ctypes
+
 import torch
 import torch.autograd.forward_ad as _fwd
 
@@ -692,13 +694,25 @@ def _rows(name, lists, read):
     return rows, dev
 
 
+def state_ptr(name, state, index):
+    """pointer of a device-side snr_step_state (None: NULL), or of whatever else holds its bytes on device number ``index``"""
+    if state is None:
+        return None
+    at = state.get_device()
+    if at >= 0 and at != index:
+        raise ValueError(f"{name}: expected a state on cuda:{index}, got one on cuda:{at}")
+    if state.numel() * state.element_size() < _STATE_BYTES or not state.is_contiguous() or state.data_ptr() % 8:
+        raise ValueError(f"{name}: a snr_step_state is {_STATE_BYTES} contiguous bytes on an address of 8; got {tuple(state.shape)} of {state.dtype}")
+    return ptr(state)
+
+
+_STATE_BYTES = ctypes.sizeof(_lib.StepState)
 # what was written through raw pointers counts as modified in place, for autograd's saved tensors and a network's packed weights
 _modified = torch.autograd.graph.increment_version
 
 
 def _items(struct, values):
     """an array of a C struct whose fields are all 8 bytes, from them one after the other"""
-    import ctypes
     flat = (ctypes.c_int64 * len(values))(*values)
     return (struct * (len(values) // len(struct._fields_))).from_buffer(flat)
 
@@ -726,7 +740,7 @@ def adam_step_multi_(params, grads, exp_avgs, exp_avg_sqs, lr, step, beta1=0.9, 
     items = _items(_lib.AdamItem, [x for p, g, m, v in rows for x in (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel())])
     with _on(dev):
         st = lib.snr_adam_step_multi(items, len(rows), float(lr), float(beta1), float(beta2), float(eps), int(step), float(grad_scale),
-                                     ptr(state), stream())
+                                     state_ptr("adam_step_multi_", state, dev), stream())
     if st:
         _no_overlap("adam_step_multi_", rows, 1)
         check(st, "snr_adam_step_multi")
@@ -878,7 +892,8 @@ def muon_step_(params, grads, momentum_buffers, lr, momentum=0.95, nesterov=True
             check(int(nbytes), "snr_muon_ws_bytes")
         ws = torch.empty(nbytes, device=rows[0][0].device, dtype=torch.uint8)
         st = lib.snr_muon_step_multi(items, len(rows), float(lr), float(momentum), int(bool(nesterov)), float(weight_decay),
-                                     _MUON_SCALE[scale], n_steps, a, b, c, eps, float(grad_scale), prec, ptr(state), ptr(ws), stream())
+                                     _MUON_SCALE[scale], n_steps, a, b, c, eps, float(grad_scale), prec,
+                                     state_ptr("muon_step_", state, dev), ptr(ws), stream())
     if st:
         _no_overlap("muon_step_", rows, 1)
         _orth_check(st, "muon_step_", "snr_muon_step_multi")
