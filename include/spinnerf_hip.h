@@ -399,7 +399,8 @@ int snr_adam_step_multi(const snr_adam_item* items, int n_items, float lr, float
 
 /* ---- orthogonalised updates (Newton-Schulz products), for the hidden matrices of a network ----
  * out = X_steps with X_0 = x / max(|x|_F, eps), A = X X^T, X <- a X + (b A + c A A) X, for every matrix of a stack [batch, rows,
- * cols] of fp32 / fp16 / bf16 whose columns are contiguous (row and matrix strides in elements).  `out` may be x itself.
+ * cols] of fp32 / fp16 / bf16 whose columns are contiguous (row and matrix strides in elements).  `out` may be x itself;
+ * that of more than one matrix must not touch x otherwise (SNR_ERR_SHAPE).
  * precision: SNR_ORTH_FP32 carries every product at fp32's accuracy, SNR_ORTH_FP16 multiplies fp16 roundings (2^-11) with fp32
  * sums (where the shorter side is above 64: below, both are the same); X itself has 22 bits in either.  a, b, c must keep singular
  * values from [0, 1] below 8 over `steps`, and |b l + c l^2| below 64 on the way (SNR_ERR_UNSUPPORTED otherwise).  A matrix that is all

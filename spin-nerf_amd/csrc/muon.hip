@@ -955,6 +955,16 @@ static bool orth_bounded(int steps, double a, double b, double c) {
   return true;
 }
 
+// Whether matrices of a stack may be overwritten before they are read: where `out` touches x without being it.  A matrix is read before
+// its own result is written, whatever its route.
+static bool stack_clash(const void* x, const void* out, int bytes, int64_t batch, int64_t m, int64_t n, int64_t xb, int64_t xr, int64_t ob, int64_t orow) {
+  if (batch == 1 || (x == out && xb == ob && (m == 1 || xr == orow))) return false;
+  const int64_t lo = (xb < 0 ? (batch - 1) * xb : 0) + (xr < 0 ? (m - 1) * xr : 0);
+  const int64_t hi = (xb > 0 ? (batch - 1) * xb : 0) + (xr > 0 ? (m - 1) * xr : 0) + n, end = (batch - 1) * ob + (m - 1) * orow + n;
+  const int64_t a = (int64_t)(uintptr_t)x, b = (int64_t)(uintptr_t)out;
+  return a + lo * bytes < b + end * bytes && b < a + hi * bytes;
+}
+
 static int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 static const int64_t kMaxSide = 65536, kMaxBatch = 65536;
 static const int64_t kMaxBlocks = 1 << 22;      // a launch is at most 2^32 threads, 1024 a workgroup
@@ -1169,6 +1179,7 @@ extern "C" int snr_orthogonalise(const void* x, int dtype, int64_t batch, int64_
   SNR_CHECK_ARG(stack_ok(batch, rows, cols) == SNR_OK && steps >= 1 && steps <= 100 && eps >= 1e-30f, SNR_ERR_SHAPE);
   SNR_CHECK_ARG(out_row_stride >= cols && (batch == 1 || out_batch_stride >= (rows - 1) * out_row_stride + cols), SNR_ERR_SHAPE);
   SNR_CHECK_ARG(dtype == SNR_F32 || dtype == SNR_F16 || dtype == SNR_BF16, SNR_ERR_UNSUPPORTED);
+  SNR_CHECK_ARG(!stack_clash(x, out, dtype == SNR_F32 ? 4 : 2, batch, rows, cols, x_batch_stride, x_row_stride, out_batch_stride, out_row_stride), SNR_ERR_SHAPE);
   SNR_CHECK_ARG(precision == SNR_ORTH_FP16 || precision == SNR_ORTH_FP32, SNR_ERR_UNSUPPORTED);
   SNR_CHECK_ARG(orth_bounded(steps, a, b, c), SNR_ERR_UNSUPPORTED);
   OrthArgs A{};
