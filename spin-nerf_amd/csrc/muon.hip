@@ -1265,9 +1265,15 @@ extern "C" int snr_muon_step_multi(const snr_muon_item* items, int n_items, floa
   SNR_CHECK_ARG(precision == SNR_ORTH_FP16 || precision == SNR_ORTH_FP32, SNR_ERR_UNSUPPORTED);
   SNR_CHECK_ARG(scale_mode == SNR_MUON_NONE || scale_mode == SNR_MUON_SPECTRAL || scale_mode == SNR_MUON_RMS, SNR_ERR_UNSUPPORTED);
   SNR_CHECK_ARG(orth_bounded(steps, a, b, c), SNR_ERR_UNSUPPORTED);
+  int64_t tiles = 0;
   for (int i = 0; i < n_items; ++i) {
     SNR_CHECK_ARG(items[i].params && items[i].grads && items[i].momentum, SNR_ERR_NULL);
     SNR_CHECK_ARG(stack_ok(items[i].batch, items[i].rows, items[i].cols) == SNR_OK, SNR_ERR_SHAPE);
+    tiles += items[i].batch * ((items[i].rows + kPad - 1) / kPad) * ((items[i].cols + kPad - 1) / kPad);
+  }
+  if (tiles > kMaxBlocks) {                    // a later sequence may be too large: all are planned before the first is launched
+    const int64_t bytes = snr_muon_ws_bytes(items, n_items, precision);
+    if (bytes < 0) return (int)bytes;
   }
   Span* spans = (Span*)malloc(sizeof(Span) * 3 * (size_t)n_items);
   if (!spans) return (int)hipErrorOutOfMemory;

@@ -27,3 +27,14 @@ def test_out_is_x_or_shares_nothing_with_a_stack(L):
                        (at, at, dict(m=1, n=64, xr=8, orow=64)), (at, at, dict(m=1, n=64, xr=100, orow=64)),      # one row: its stride says nothing
                        (at, at + 32, dict(batch=1)), (at, at, dict(batch=1, xb=7))):                                # one matrix is read before it is written
         assert orth(x, out, **kw) == UNSUPPORTED, (x - at, out - at, kw)
+
+
+def test_a_step_that_is_refused_has_not_begun(L):
+    """300 matrices of 8 x 8 are a launch of their own, ahead of the 4097 whose grid would be too large"""
+    lib = L.load()
+    small, large = L.MuonItem(1 << 20, 1 << 24, 1 << 28, 300, 8, 8), L.MuonItem(1 << 40, 1 << 42, 1 << 44, 4097, 1, 65536)
+
+    def muon(items):
+        return lib.snr_muon_step_multi((L.MuonItem * len(items))(*items), len(items), 1e-3, 0.95, 1, 0.0, 1, 5, 3.4445, -4.775, 2.0315, 1e-7, 1.0,
+                                       0, None, 1 << 30, None)
+    assert muon([large]) == SHAPE and muon([small, large]) == SHAPE and muon([large, small]) == SHAPE
