@@ -632,20 +632,22 @@ class RenderTrainer:
     def load_state_dict(self, ckpt):
         """Accepts checkpoints written by save_checkpoint() or by the reference's train()."""
         fn, fine = self.kw.get('network_fn'), self.kw.get('network_fine')
+        osd = ckpt['optimizer_state_dict']
+        st = osd['state']
+        from .render import scatter_per_layer_adam
+        # what the optimizer state refuses is refused ahead of every change
+        moments = [(torch.zeros_like(m), torch.zeros_like(v)) for m, v in zip(self.m, self.v)]
+        steps = set(scatter_per_layer_adam(st, self.nets, moments, muon=self.muon is not None)) if st else set()
+        steps.discard(0.0) if len(steps) > 1 else None      # (a network all of whose layers are idle carries no step count)
+        if len(steps) > 1:
+            raise RuntimeError(f"checkpoint parameters disagree on the Adam step count: {sorted(steps)}")
         if fn is not None:
             fn.load_state_dict(ckpt['network_fn_state_dict'])
         if fine is not None and ckpt.get('network_fine_state_dict') is not None:
             fine.load_state_dict(ckpt['network_fine_state_dict'])
+        for m, v, (m1, v1) in zip(self.m, self.v, moments):
+            m.copy_(m1); v.copy_(v1)
         self.global_step = int(ckpt['global_step'])
-        osd = ckpt['optimizer_state_dict']
-        st = osd['state']
-        from .render import scatter_per_layer_adam
-        for m, v in zip(self.m, self.v):
-            m.zero_(); v.zero_()
-        steps = set(scatter_per_layer_adam(st, self.nets, list(zip(self.m, self.v)), muon=self.muon is not None)) if st else set()
-        steps.discard(0.0) if len(steps) > 1 else None      # (a network all of whose layers are idle carries no step count)
-        if len(steps) > 1:
-            raise RuntimeError(f"checkpoint parameters disagree on the Adam step count: {sorted(steps)}")
         self.opt_step = int(steps.pop()) if steps else 0
         self._lr = float(osd['param_groups'][0]['lr']) if osd.get('param_groups') else self.lrate
         for n in self.nets:

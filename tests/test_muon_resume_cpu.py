@@ -95,3 +95,21 @@ def test_a_state_that_does_not_fit_is_refused(train, args, tmp_path):  # noqa: F
         torch.save(ck, path)
         with pytest.raises(RuntimeError, match=why):
             S.create_nerf(args, device=CPU)
+
+
+@pytest.mark.parametrize("muon", [True, None])
+def test_a_refused_checkpoint_leaves_the_trainer_as_it_was(train, args, tmp_path, monkeypatch, muon):  # noqa: F811
+    from test_checkpoint_cpu import _cpu_adam
+    monkeypatch.setattr(train.ops, "adam_step_", _cpu_adam)
+    args.no_reload = True
+    other = tmp_path / "other.tar"
+    trained(train, args, other, muon=None if muon else True)          # the other kind's
+    tr = trained(train, args, tmp_path / "own.tar", muon=muon)
+    steps(tr, (5,))
+    now = lambda: [t.detach().clone() for t in [n.flat for n in tr.nets] + tr.m + tr.v]  # noqa: E731
+    before, counts = now(), (tr.opt_step, tr.global_step, tr.current_lr())
+    with pytest.raises(RuntimeError, match="momentum buffer"):
+        tr.load_checkpoint(str(other))
+    assert all(torch.equal(a, b) for a, b in zip(before, now())) and counts == (tr.opt_step, tr.global_step, tr.current_lr())
+    tr.load_checkpoint(str(tmp_path / "own.tar"))                     # and its own loads as ever
+    assert tr.opt_step == 3 and not torch.equal(before[0], tr.nets[0].flat.detach())
