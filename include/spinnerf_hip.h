@@ -430,6 +430,13 @@ int snr_muon_step_multi(const snr_muon_item* items, int n_items, float lr, float
                         int scale_mode, int steps, float a, float b, float c, float eps, float grad_scale, int precision,
                         const snr_step_state* state, void* ws, snr_stream_t stream);
 
+/* diagnostics: the launch sequences that a list goes through (snr_orthogonalise: as a list of its one stack), in their order, three
+ * numbers each: the kind (SNR_ROUTE_*: one workgroup a matrix, or tiles), and the side of the tiles of the symmetric products and of
+ * B Y (0 without tiles).  Pointers are not looked at.  Returns how many there are; the first max_routes are written to `routes`. */
+enum { SNR_ROUTE_64x64 = 0, SNR_ROUTE_64x128, SNR_ROUTE_64x256, SNR_ROUTE_64x448, SNR_ROUTE_128x128, SNR_ROUTE_128x128_FP16,
+       SNR_ROUTE_128x192_FP16, SNR_ROUTE_128x320_FP16, SNR_ROUTE_TILES, SNR_ROUTE_TILES_FP16 };
+int snr_muon_routes(const snr_muon_item* items, int n_items, int precision, int* routes, int max_routes);
+
 /* ---- diagnostics: per-kernel HIP-event timing (used by bench.py for the roofline line) ----
  * When enabled, every kernel launch of this library is bracketed by hipEvents on its stream;
  * snr_prof_read() waits for them, returns total elapsed ms and launch count per kernel id

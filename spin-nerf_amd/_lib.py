@@ -139,6 +139,7 @@ SIGNATURES = {
     "snr_orthogonalise_ws_bytes": (_l, [_l, _l, _l, _i]),
     "snr_orthogonalise": (_i, [_p, _i, _l, _l, _l, _l, _l, _p, _l, _l, _i, _f, _f, _f, _f, _i, _p, _p]),
     "snr_muon_ws_bytes": (_l, [_c.POINTER(MuonItem), _i, _i]),
+    "snr_muon_routes": (_i, [_c.POINTER(MuonItem), _i, _i, _c.POINTER(_i), _i]),
     "snr_muon_step_multi": (_i, [_c.POINTER(MuonItem), _i, _f, _f, _i, _f, _i, _i, _f, _f, _f, _f, _f, _i, _p, _p, _p]),
     "snr_prof_enable": (_i, [_i]),
     "snr_prof_kernel_count": (_i, []),

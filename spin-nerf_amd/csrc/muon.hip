@@ -974,7 +974,7 @@ static int stack_ok(int64_t batch, int64_t m, int64_t n) {
 }
 // What a matrix goes through: one workgroup (64 or 128 rows, so many columns, split or hi planes alone), the split products of tiles, or
 // fp16 products of tiles.
-enum { kSmall64, kSmall128, kSmall256, kSmall448, kMid128, kMid128h, kMid192h, kMid320h, kSplit, kHalf, kKinds };
+enum { kSmall64 = SNR_ROUTE_64x64, kSmall128, kSmall256, kSmall448, kMid128, kMid128h, kMid192h, kMid320h, kSplit = SNR_ROUTE_TILES, kHalf, kKinds };
 static int kind_of(int precision, int64_t m, int64_t n) {
   const int64_t r = m < n ? m : n, c = m < n ? n : m;
   const bool split = precision == SNR_ORTH_FP32 || r <= 64;
@@ -1239,7 +1239,8 @@ template <class F> static int for_sequences(const snr_muon_item* items, int n_it
   return SNR_OK;
 }
 
-extern "C" int64_t snr_muon_ws_bytes(const snr_muon_item* items, int n_items, int precision) {
+// F(const OrthPlan&, kind) for each sequence that the items would take
+template <class F> static int plan_sequences(const snr_muon_item* items, int n_items, int precision, F f) {
   if (!items) return SNR_ERR_NULL;
   if (n_items < 1) return SNR_ERR_SHAPE;
   if (precision != SNR_ORTH_FP16 && precision != SNR_ORTH_FP32) return SNR_ERR_UNSUPPORTED;
@@ -1247,14 +1248,28 @@ extern "C" int64_t snr_muon_ws_bytes(const snr_muon_item* items, int n_items, in
     const int st = stack_ok(items[i].batch, items[i].rows, items[i].cols);
     if (st != SNR_OK) return st;
   }
-  int64_t most = 0;
-  const int st = for_sequences(items, n_items, precision, [&](OrthArgs& A, int kind) {
+  return for_sequences(items, n_items, precision, [&](OrthArgs& A, int kind) {
     OrthPlan p;
     const int ok = orth_plan(A, kind, p);
-    most = ok == SNR_OK && p.bytes > most ? p.bytes : most;
+    if (ok == SNR_OK) f(p, kind);
     return ok;
   });
+}
+
+extern "C" int64_t snr_muon_ws_bytes(const snr_muon_item* items, int n_items, int precision) {
+  int64_t most = 0;
+  const int st = plan_sequences(items, n_items, precision, [&](const OrthPlan& p, int) { most = p.bytes > most ? p.bytes : most; });
   return st != SNR_OK ? st : most;
+}
+
+extern "C" int snr_muon_routes(const snr_muon_item* items, int n_items, int precision, int* routes, int max_routes) {
+  if (max_routes > 0 && !routes) return SNR_ERR_NULL;
+  int n = 0;
+  const int st = plan_sequences(items, n_items, precision, [&](const OrthPlan& p, int kind) {
+    if (n < max_routes) { routes[3 * n] = kind; routes[3 * n + 1] = kind < kSplit ? 0 : p.ts; routes[3 * n + 2] = kind < kSplit ? 0 : p.tf; }
+    ++n;
+  });
+  return st != SNR_OK ? st : n;
 }
 
 extern "C" int snr_muon_step_multi(const snr_muon_item* items, int n_items, float lr, float momentum, int nesterov, float weight_decay,
