@@ -402,8 +402,9 @@ int snr_adam_step_multi(const snr_adam_item* items, int n_items, float lr, float
  * cols] of fp32 / fp16 / bf16 whose columns are contiguous (row and matrix strides in elements).  `out` may be x itself;
  * that of more than one matrix must not touch x otherwise (SNR_ERR_SHAPE).
  * precision: SNR_ORTH_FP32 carries every product at fp32's accuracy, SNR_ORTH_FP16 multiplies fp16 roundings (2^-11) with fp32
- * sums (where the shorter side is above 64: below, both are the same); X itself has 22 bits in either.  a, b, c must keep singular
- * values from [0, 1] below 8 over `steps`, and |b l + c l^2| below 64 on the way (SNR_ERR_UNSUPPORTED otherwise).  A matrix that is all
+ * sums (where the shorter side is above 64: below, both are the same); X itself is kept to 2^-23 of an entry in either, or to 2^-46 of
+ * max(|x|_F, eps) where that is more.  a, b, c must keep singular values from [0, 1] below 8 over `steps`, and |b l + c l^2| below 64 on
+ * the way (SNR_ERR_UNSUPPORTED otherwise).  A matrix that is all
  * zero gives zeros; one with a NaN or an infinity gives NaN throughout.  A call repeats bit for bit; how much else it has to do
  * chooses tiles, and with them a result's last bits.  Sides and batch up to 65536 (SNR_ERR_SHAPE). */
 enum { SNR_F32 = 0, SNR_F16 = 1, SNR_BF16 = 2 };

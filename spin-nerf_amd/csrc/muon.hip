@@ -6,7 +6,8 @@
 // Y [r x c] with r <= c and the Gram matrix A is r x r.
 //
 // Numbers.  Y, A and B = b A + c A^2 are held as hi + 2^-11 lo, two fp16 planes (22 mantissa bits, as much memory as fp32), each
-// scaled by a power of two so that fp16's range covers what a polynomial that stays bounded can reach (orth_bounded below).
+// scaled by a power of two so that fp16's range covers what a polynomial that stays bounded can reach (orth_bounded below); at the
+// other end an entry of Y below 2^-24 keeps 2^-46 absolutely, fp16's subnormals over both scales.
 // SNR_ORTH_FP32 multiplies hi hi + hi lo + lo hi (three v_mfma_f32_32x32x16_f16; the dropped lo lo is 2^-24 of a product): fp32's
 // accuracy at a third of the fp16 rate, 5 x the fp32 matrix rate.  SNR_ORTH_FP16 multiplies the hi planes only, except where the
 // shorter side is 64 or less: there the roundings of a direction's few entries do not average out (up to 1 % of a singular value
