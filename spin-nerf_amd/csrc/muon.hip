@@ -306,9 +306,10 @@ __global__ __launch_bounds__(256) void orth_split_kernel(const OrthArgs* __restr
 //
 // What bounds them.  A launch costs some 5 us however little it has to do (2 x 128 x 283: 6.5 us a product), plus a tile's first
 // slices and its epilogue; then a compute unit takes in about 88 B / ns by DMA (128-wide tiles: 32 KB and 0.37 us a slice), which is
-// what larger tiles are for, and what the products themselves reach with the whole chip on random data is 0.92 PF (4096^2, 192 and
-// 256 wide; a large library product: 1.33 PF, and zeros instead of data run 1.3 .. 1.5 x faster here: power).  Halving the fragments'
-// reads from LDS changes nothing, nor does the order of the tiles.
+// what larger tiles are for; below that, compute units without a tile (136 of 128 a symmetric product of 2048^2: 120 idle, 0.6 PF); and
+// with the whole chip busy, power: 4096^2 runs at 0.92 PF in all, B Y (256 wide) at 1.0, where a library product of the same size and
+// data reaches 0.99 and one of zeros 1.5 (fp16; 8192^3: 1.30 and 1.8).  Halving the fragments' reads from LDS changes nothing, nor does
+// the order of the tiles.
 enum { kGram = 0, kPoly = 1, kApply = 2 };   // template PHASE; LAST: the result instead of planes
 
 template <int T_, int WI_, int WJ_, bool SPLIT_, int STAGES_, int BK_> struct TileCfg {
@@ -711,9 +712,11 @@ __global__ __launch_bounds__(C::NT) void orth_product_kernel(OrthHead h, OrthOut
 // ---- 4. small matrices: everything in one workgroup ----------------------------------------------------------------------------------
 // Where a matrix fits, a workgroup keeps it from its input to its result: 17 launches of a microsecond's work each become one.  Y stays in
 // registers in 32 bits, as 32 x 32 blocks in the layout the matrix instructions give them back in (NB a wave; a wave's block never
-// moves); LDS holds the planes that all waves multiply from: 32 RB rows, 64 NB columns, hi and lo (SPLIT) or hi alone.  What fits
-// 160 KB beside A and B: 64 x 448 and 128 x 128 split, 128 x 320 else.  Bound by the latency of a few rounds of LDS reads and products
-// between four barriers a step, then by LDS.  Us a call, here / in tiles: 2 x 128 x 283 fp16 47 / 82, 2 x 128 x 128 fp16 29 / 70,
+// moves); LDS holds the planes that all waves multiply from: 32 RB rows, 64 NB columns, hi and lo (SPLIT) or hi alone.  As many columns
+// as fit 160 KB beside A, with B in A's place where there is no room for both: 64 x 448 and 128 x 128 split.  128 x 384 of hi planes
+// would fit, but not the 256 registers that 8 waves leave each other: 61 of them would be spilled; 128 x 320, and 128 x 128 split, spill 7
+// outside the products' loops.  Bound by the latency of a few rounds of LDS reads and products between four barriers a step, then by
+// LDS; two matrices use two compute units.  Us a call, here / in tiles: 2 x 128 x 283 fp16 47 / 82, 2 x 128 x 128 fp16 29 / 70,
 // fp32 57 / 84; 1024 x 128 x 128 fp16 120 / 538, fp32 242 / 708; 64 x 64: 17 (what calling it takes), 64 x 448: 52.
 template <int RB, int NB, bool SPLIT>
 __global__ __launch_bounds__(128 * RB) void orth_small_kernel(OrthArgs a, OrthOut o, float ca, float cb, float cc, int steps) {
